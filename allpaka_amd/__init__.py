@@ -9,4 +9,4 @@ memory.  There is no CPU fallback: without the built library every entry
 raises.
 """
 from .lib import ApkError, Declined, load, lib_path  # noqa: F401
-from .backend import Backend, QuantMat, Gating, GgmlType  # noqa: F401
+from .backend import Backend, PagedCache, QuantMat, Gating, GgmlType  # noqa: F401

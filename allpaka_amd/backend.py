@@ -143,6 +143,13 @@ class Backend:
         if not self._recording:
             self.sync()
 
+    def _order(self):
+        """For the enqueue-only entries: the context's stream runs after what torch has queued.  The context's stream and the
+        default stream order themselves against each other; any other stream of torch's is waited for."""
+        cur = torch.cuda.current_stream(self.device)
+        if self._recording or cur.cuda_stream not in (0, self.L.apk_stream(self.h)):
+            cur.synchronize()
+
     # ---- record / replay (stream capture of gpu/cuda/prefill.rs:52-108)
     def capture_begin(self):
         self._enter()
@@ -567,6 +574,154 @@ class Backend:
         assert logits.dtype == torch.float32 and out.dtype == torch.int32 and out.numel() >= rows
         self._enter()
         check(self.L.apk_argmax_rows(self.h, _ptr(logits), rows, n, _ptr(out)))
+
+
+    # ---- attention over the paged cache (gpu::attend / attend_batch, gpu/stub.rs)
+    def _attend_check(self, q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, out, window):
+        assert q.dim() == 2 and q.shape[1] == n_q * head_dim and out.shape == q.shape and out.dtype == q.dtype
+        assert k_cache.dtype == v_cache.dtype == torch.float16 and k_cache.shape == v_cache.shape
+        assert k_cache.dim() == 2 and k_cache.shape[1] == n_kv * head_dim
+        assert page_table.dtype == kv_len.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == kv_len.numel()
+        assert page_size >= 1 and window >= 0
+        for t in (q, k_cache, v_cache, page_table, kv_len, out):
+            assert t.device == self.device, "a tensor of another device"
+
+    def attend_paged_into(self, q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, scale, out, window=0):
+        """Attention of one new token per sequence over the paged cache: q, out [n_seq, n_q*head_dim]; k_cache, v_cache fp16
+        [capacity, n_kv*head_dim], page p the rows [p*page_size, (p+1)*page_size); page_table int32 [n_seq, max_pages];
+        kv_len int32 [n_seq], the token itself included; window: keys a row sees (0: all).  Enqueued only (no wait)."""
+        self._attend_check(q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, out, window)
+        assert q.shape[0] == kv_len.numel()
+        self._order()
+        check(self.L.apk_attend_paged(self.h, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], page_size, _ptr(page_table),
+                                      page_table.shape[1], _ptr(kv_len), kv_len.numel(), n_q, n_kv, head_dim, scale, window, _ptr(out), _dt(q)))
+
+    def attend_paged(self, q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, scale, window=0):
+        """attend_paged_into a tensor of its own, waited for."""
+        out = torch.empty_like(q)
+        self._enter()
+        self.attend_paged_into(q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, scale, out, window)
+        self._leave()
+        return out
+
+    def attend_paged_chunk_into(self, q, k_cache, v_cache, page_size, page_table, q_off, kv_len, n_q, n_kv, head_dim, scale, out, window=0):
+        """The same for chunks: sequence s brings the rows q_off[s]:q_off[s+1] of q (int32 [n_seq+1]), its newest tokens; rows
+        at and behind q_off[n_seq] of out are left as they are.  Enqueued only (no wait)."""
+        self._attend_check(q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, out, window)
+        assert q_off.dtype == torch.int32 and q_off.numel() == kv_len.numel() + 1 and q_off.device == self.device
+        self._order()
+        check(self.L.apk_attend_paged_chunk(self.h, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], page_size, _ptr(page_table),
+                                            page_table.shape[1], _ptr(q_off), _ptr(kv_len), kv_len.numel(), q.shape[0], n_q, n_kv, head_dim,
+                                            scale, window, _ptr(out), _dt(q)))
+
+    def attend_paged_chunk(self, q, k_cache, v_cache, page_size, page_table, q_off, kv_len, n_q, n_kv, head_dim, scale, window=0):
+        """attend_paged_chunk_into a tensor of zeros, waited for."""
+        out = torch.zeros_like(q)
+        self._enter()
+        self.attend_paged_chunk_into(q, k_cache, v_cache, page_size, page_table, q_off, kv_len, n_q, n_kv, head_dim, scale, out, window)
+        self._leave()
+        return out
+
+
+class PageStep:
+    """What one PagedCache.extend hands out: the rows of every sequence (q_off), their positions and cache rows (slots)."""
+
+    def __init__(self, n_seq, rows, device):
+        def buf(*shape):
+            return torch.empty(shape, dtype=torch.int32, device=device)
+
+        self.q_off, self.positions, self.slots = buf(n_seq + 1), buf(rows), buf(rows)
+        self.pairs, self.n_pairs = buf(max(n_seq, 1), 2), buf(1)
+
+
+class PagedCache:
+    """A K/V cache shared by many sequences: region fp16 [n_planes, capacity, n_kv*head_dim] (the K and V planes of all
+    layers), in pages of page_size rows, with the page table and the lengths of n_seq sequences on the device.  The
+    methods are enqueued only, in stream order, and may be recorded (the buffers of a PageStep given to extend)."""
+
+    def __init__(self, backend, region, page_size, n_seq, max_pages):
+        assert region.dtype == torch.float16 and region.dim() == 3 and region.is_contiguous() and region.device == backend.device
+        assert page_size >= 1 and region.shape[1] // page_size >= 1
+        self.b, self.region, self.page_size = backend, region, page_size
+        self.n_pages, self.n_seq, self.max_pages = region.shape[1] // page_size, n_seq, max_pages
+        dev = backend.device
+        self.pool = torch.zeros(backend.L.apk_pages_words(self.n_pages), dtype=torch.int32, device=dev)
+        self.page_table = torch.full((n_seq, max_pages), -1, dtype=torch.int32, device=dev)
+        self.kv_len = torch.zeros(n_seq, dtype=torch.int32, device=dev)
+        self._moves = torch.empty((max(self.n_pages // 2, 1), 2), dtype=torch.int32, device=dev)
+        self._n_moves = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._recount()
+
+    def _state(self):
+        return (self.b.h, _ptr(self.pool), self.n_pages, self.page_size, _ptr(self.page_table), self.max_pages, _ptr(self.kv_len), self.n_seq)
+
+    def _recount(self):
+        self.b._order()
+        check(self.b.L.apk_pages_init(*self._state()))
+
+    @property
+    def refs(self):
+        """The holders of every page, int32 [n_pages]."""
+        return self.pool[4:4 + self.n_pages]
+
+    @property
+    def free_pages(self):
+        """The number of free pages (waits)."""
+        self.b.sync()
+        return int(self.pool[0].item())
+
+    def adopt(self, page_table, kv_len):
+        """Takes over tables filled elsewhere; the pool is counted afresh."""
+        assert page_table.shape == self.page_table.shape and kv_len.shape == self.kv_len.shape
+        self.page_table.copy_(page_table)
+        self.kv_len.copy_(kv_len)
+        self._recount()
+
+    def save(self):
+        """The state (not the cache rows) as copies, for restore."""
+        self.b.sync()
+        return self.pool.clone(), self.page_table.clone(), self.kv_len.clone()
+
+    def restore(self, saved):
+        for t, s in zip((self.pool, self.page_table, self.kv_len), saved):
+            t.copy_(s)
+
+    def _ids(self, t, n=None):
+        assert t.dtype == torch.int32 and t.device == self.b.device and (n is None or t.numel() == n)
+        return _ptr(t)
+
+    def extend(self, n_new, rows, step=None):
+        """n_new int32 [n_seq] more tokens; rows: the most there can be in all.  Shared pages that get written to are copied
+        in every plane.  Returns the PageStep (step: one to fill, of this n_seq and rows)."""
+        step = PageStep(self.n_seq, rows, self.b.device) if step is None else step
+        assert step.positions.numel() == rows and step.q_off.numel() == self.n_seq + 1
+        self.b._order()
+        check(self.b.L.apk_pages_extend(*self._state(), self._ids(n_new, self.n_seq), rows, _ptr(step.q_off), _ptr(step.positions),
+                                        _ptr(step.slots), _ptr(step.pairs), _ptr(step.n_pairs)))
+        self._copy(step.pairs, step.n_pairs, self.n_seq)
+        return step
+
+    def fork(self, src, dst):
+        """Sequences dst (holding nothing) become further holders of the pages of sequences src."""
+        assert src.numel() == dst.numel()
+        self.b._order()
+        check(self.b.L.apk_pages_fork(*self._state(), self._ids(src), self._ids(dst), src.numel()))
+
+    def truncate(self, new_len):
+        """Cuts sequences to new_len int32 [n_seq] tokens; -1 leaves one as it is, 0 frees it."""
+        self.b._order()
+        check(self.b.L.apk_pages_truncate(*self._state(), self._ids(new_len, self.n_seq)))
+
+    def compact(self):
+        """Moves the pages in use to the front of every plane."""
+        self.b._order()
+        check(self.b.L.apk_pages_compact(*self._state(), _ptr(self._moves), _ptr(self._n_moves)))
+        self._copy(self._moves, self._n_moves, max(self.n_pages // 2, 1))
+
+    def _copy(self, pairs, n_pairs, most):
+        planes, capacity, width = self.region.shape
+        check(self.b.L.apk_pages_copy(self.b.h, _ptr(self.region), planes, capacity * width * 2, self.n_pages, self.page_size * width * 2,
+                                      _ptr(pairs), _ptr(n_pairs), most))
 
 
 class _Recording:

@@ -5,6 +5,7 @@
 // failing, and hipModuleLaunchKernel.  No device code in this translation unit:
 // it builds with a plain host C++ compiler against the HIP runtime API.
 #include "apk_hip.h"
+#include "apk_attend.h"
 #include "apk_internal.h"
 
 #include <hip/hip_runtime_api.h>
@@ -65,6 +66,7 @@ const int kAddnormTiles[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20};  // 16-byte t
 const int kAddnormBound[] = {1024, 1024, 512, 512, 256, 256, 256, 256, 256, 256, 256};  // launch bound of each
 const int kQkIters[] = {1};
 const int kQkHeadDims[] = {64, 128, 256};
+const int kAttendHeadDims[] = {64, 128, 256};
 
 std::vector<std::string> all_kernel_names() {
     std::vector<std::string> v = {"apk_swiglu_f32", "apk_swiglu_f16", "apk_geglu_tanh_f32", "apk_geglu_tanh_f16", "apk_rope_table", "apk_embed_q4k_f32",
@@ -72,8 +74,15 @@ std::vector<std::string> all_kernel_names() {
                                   "apk_moe_permute", "apk_gather_rows", "apk_scatter_rows_t1", "apk_scatter_rows_t2", "apk_argmax_rows", "apk_add_rmsnorm_ragged_f32", "apk_add_rmsnorm_ragged_f16", "apk_copy",
                                   "apk_qknorm_rope_generic_f32", "apk_qknorm_rope_generic_f16", "apk_qknorm_rope_pos_f32", "apk_qknorm_rope_pos_f16", "apk_route_topk_wide", "apk_route_topk_e64", "apk_route_topk_e128", "apk_route_group_small_e64", "apk_route_group_small_e128",
                                   "apk_route_group_small_e256", "apk_route_group_small_e1024", "apk_add_assign_f32", "apk_add_assign_f16", "apk_add_scaled_f32", "apk_add_scaled_f16", "apk_softmax_rows", "apk_moe_count", "apk_moe_rank",
-                                  "apk_add_bias_rows_f32", "apk_add_bias_rows_f16", "apk_moe_shared_hits", "apk_cast_f32_f16", "apk_cast_f16_f32", "apk_zero_u64"};
+                                  "apk_add_bias_rows_f32", "apk_add_bias_rows_f16", "apk_moe_shared_hits", "apk_cast_f32_f16", "apk_cast_f16_f32", "apk_zero_u64",
+                                  "apk_pages_init_k", "apk_pages_extend_k", "apk_pages_fork_k", "apk_pages_truncate_k", "apk_pages_compact_k", "apk_pages_copy_k"};
     for (const char* t : {"f32", "f16"}) {
+        for (int hd : kAttendHeadDims) {
+            v.push_back(std::string("apk_attend_token_") + t + "_hd" + std::to_string(hd) + "_w4");
+            v.push_back(std::string("apk_attend_chunk_") + t + "_hd" + std::to_string(hd));
+        }
+        for (const char* w : {"_w1", "_w4"}) v.push_back(std::string("apk_attend_join_") + t + w);
+        v.push_back(std::string("apk_attend_any_") + t);
         for (const char* f : {"q5k", "q6k", "q2k", "q3k", "q5_0", "f16", "f32", "bf16"}) v.push_back(std::string("apk_embed_") + f + "_" + t);
         for (int c : kAddnormTiles) v.push_back(std::string("apk_add_rmsnorm_") + t + "_c" + std::to_string(c));
         for (int c : kAddnormTiles) v.push_back(std::string("apk_postnorm_add_rmsnorm_") + t + "_c" + std::to_string(c));
@@ -114,6 +123,7 @@ struct apk_ctx {
     size_t permute_counts_cap = 0;       // in u32
     bool capture_permute = false;
     size_t graphs_with_permute = 0;
+    void* attend_part = nullptr;  // kAttendScratch bytes: the partial results of attention whose keys are split
     std::set<apk_graph*> live_graphs;  // recorded graphs not yet destroyed: they hold device addresses, also inside attached mappings
     uint64_t clock = 0;  // counts attaches that copied and recordings that ended: orders a graph against a mapping
     std::mutex mu;
@@ -564,6 +574,7 @@ int apk_shutdown(apk_ctx* c) {
     if (c->fault_dev) (void)hipFree(c->fault_dev);
     if (c->argmax_scratch) (void)hipFree(c->argmax_scratch);
     if (c->permute_counts) (void)hipFree(c->permute_counts);
+    if (c->attend_part) (void)hipFree(c->attend_part);
     if (c->ev0) (void)hipEventDestroy(c->ev0);
     if (c->ev1) (void)hipEventDestroy(c->ev1);
     if (c->stream) (void)hipStreamDestroy(c->stream);
@@ -1562,6 +1573,226 @@ int apk_argmax_rows(apk_ctx* c, const float* logits, size_t rows, size_t n, uint
     }
     if (c->capturing) c->capture_argmax = true;
     return argmax_locked(c, logits, rows, n, out, c->argmax_scratch, false);
+}
+
+/* ---------------------------------------------------------- the paged cache */
+
+namespace {
+
+const size_t kAttendScratch = 256u << 20;
+
+// page / key arithmetic of the kernels: floor(2^32 / page), 2^32 - 1 for page 1
+uint32_t page_magic(size_t page) { return page == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / page); }
+
+// What both attention entries check and launch.  q_off NULL: one row per sequence.
+int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, const void* v_cache, size_t capacity, size_t page_size,
+           const uint32_t* page_table, size_t max_pages, const uint32_t* q_off, const uint32_t* kv_len, size_t n_seq, size_t rows,
+           size_t n_q, size_t n_kv, size_t head_dim, float scale, size_t window, void* out, int dtype) {
+    const int es = elem_size(dtype);
+    if (!es) return fail(APK_DECLINE_UNSUPPORTED, "%s: dtype %d", name, dtype);
+    if (n_q == 0 || n_kv == 0 || n_q % n_kv || n_q > 65535) return fail(APK_DECLINE_SHAPE, "%s: n_q %zu, n_kv %zu", name, n_q, n_kv);
+    if (head_dim == 0 || head_dim > 1024) return fail(APK_DECLINE_UNSUPPORTED, "%s: head_dim %zu (1..1024)", name, head_dim);
+    if (!(scale - scale == 0.f)) return fail(APK_DECLINE_SHAPE, "%s: scale is not finite", name);
+    if (page_size == 0 || capacity < page_size || capacity > 0xffffffffu)
+        return fail(APK_DECLINE_SHAPE, "%s: page_size %zu, capacity %zu", name, page_size, capacity);
+    if (max_pages == 0 || max_pages > (1u << 30) || page_size > (1u << 30) || max_pages * page_size > (1u << 30))
+        return fail(APK_DECLINE_SHAPE, "%s: max_pages %zu * page_size %zu (1..2^30)", name, max_pages, page_size);
+    if (n_seq == 0 || rows == 0) return APK_OK;
+    if (n_seq > 0x7fffffffu || rows > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
+    if (!q || !k_cache || !v_cache || !page_table || !kv_len || !out) return fail(APK_DECLINE_NULL, "%s: NULL tensor", name);
+    if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+        return fail(APK_DECLINE_SHAPE, "%s: tensors must be 16-byte aligned", name);
+    apk_attend_args a;
+    memset(&a, 0, sizeof a);
+    a.q = q;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.out = out;
+    a.table = page_table;
+    a.q_off = q_off;
+    a.kv_len = kv_len;
+    a.fault = c->fault_dev;
+    a.n_seq = (uint32_t)n_seq;
+    a.rows = (uint32_t)rows;
+    a.n_q = (uint32_t)n_q;
+    a.n_kv = (uint32_t)n_kv;
+    a.hd = (uint32_t)head_dim;
+    a.group = (uint32_t)(n_q / n_kv);
+    a.page = (uint32_t)page_size;
+    a.page_magic = page_magic(page_size);
+    a.max_pages = (uint32_t)max_pages;
+    a.n_pages = (uint32_t)(capacity / page_size);
+    a.window = window >= max_pages * page_size ? 0 : (uint32_t)window;
+    a.c = fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f);  // above zero: a masked score stays -inf when multiplied by it
+    a.sign = scale < 0.f ? -1.f : 1.f;
+    a.head_tiles = 1;
+    const std::string t = dtype == APK_F32 ? "f32" : "f16";
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
+        if (rows * n_q > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
+        if (int rc = set_device(c)) return rc;
+        void* args[] = {&a};
+        return launch(c, "apk_attend_any_" + t, (unsigned)(rows * n_q), 256, (unsigned)((5 * head_dim + 8) * 4), args);
+    }
+    unsigned shmem;
+    uint64_t tiles;
+    std::string kernel;
+    if (!q_off) {
+        a.tile_rows = APK_ATT_TOKEN_ROWS;
+        a.unit = APK_ATT_TOKEN_UNIT;
+        a.head_tiles = (a.group + APK_ATT_TOKEN_ROWS - 1) / APK_ATT_TOKEN_ROWS;
+        a.target = 1024;
+        a.unit_min = 2;
+        tiles = n_seq;
+        const unsigned r = a.group < APK_ATT_TOKEN_ROWS ? a.group : APK_ATT_TOKEN_ROWS;
+        shmem = (unsigned)((2 * 4 * 16 + 4 * r * head_dim) * 4);
+        kernel = "apk_attend_token_" + t + "_hd" + std::to_string(head_dim) + "_w4";
+    } else {
+        a.tile_rows = APK_ATT_CHUNK_ROWS;
+        a.unit = head_dim == 256 ? 32 : APK_ATT_CHUNK_UNIT;
+        a.target = 512;
+        a.unit_min = 512 / a.unit;
+        tiles = rows * (uint64_t)a.group / APK_ATT_CHUNK_ROWS + n_seq;
+        shmem = (unsigned)(4 * a.unit * head_dim * 2);
+        kernel = "apk_attend_chunk_" + t + "_hd" + std::to_string(head_dim);
+    }
+    // slots never exceed 2 * target: a cut tile has at least two parts, of more than half of a part's share of all units
+    const size_t slot = (size_t)a.tile_rows * (head_dim + 2) * 4;
+    if (2 * (size_t)a.target * slot > kAttendScratch) a.target = (uint32_t)(kAttendScratch / (2 * slot));
+    const uint64_t H = (uint64_t)n_kv * a.head_tiles;
+    const uint64_t units = (max_pages * page_size + a.unit - 1) / a.unit;
+    const uint64_t parts = units > a.unit_min ? (units + a.unit_min - 1) / a.unit_min : 1;  // of a tile at most
+    uint64_t items = tiles + (a.target + H - 1) / H + 1;
+    if (parts < items && tiles * parts < items) items = tiles * parts;
+    if (items * H > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
+    if (int rc = set_device(c)) return rc;
+    if (parts > 1 && !c->attend_part) {
+        if (c->capturing) return fail(APK_DECLINE_CAPTURE, "%s: the scratch would have to be allocated inside a recording (run once unrecorded first)", name);
+        HIP_TRY(hipMalloc(&c->attend_part, kAttendScratch));
+    }
+    a.part = (float*)c->attend_part;
+    void* args[] = {&a};
+    if (int rc = launch(c, kernel, (unsigned)(items * H), 256, shmem, args)) return rc;
+    if (parts == 1) return APK_OK;
+    uint64_t cut = tiles * H < a.target ? tiles * H : a.target;  // tiles that may have been cut
+    cut = (cut + H - 1) / H * H;
+    if (q_off) return launch(c, "apk_attend_join_" + t + "_w1", (unsigned)(cut * (a.tile_rows / 4)), 256, 0, args);
+    return launch(c, "apk_attend_join_" + t + "_w4", (unsigned)(cut * a.tile_rows), 256, 0, args);
+}
+
+// The checks that the page entries share.
+int pages_check(const char* name, apk_ctx* c, const uint32_t* pool, size_t n_pages, size_t page_size, const uint32_t* page_table,
+                size_t max_pages, const uint32_t* kv_len, size_t n_seq) {
+    if (!c) return fail(APK_DECLINE_NULL, "%s: ctx is NULL", name);
+    if (!pool || (n_seq && (!page_table || !kv_len))) return fail(APK_DECLINE_NULL, "%s: NULL tensor", name);
+    if (n_pages == 0 || page_size == 0 || n_pages > 0xffffffffu / page_size || n_pages > (1u << 28))
+        return fail(APK_DECLINE_SHAPE, "%s: n_pages %zu, page_size %zu", name, n_pages, page_size);
+    if (n_seq > (1u << 24) || (n_seq && (max_pages == 0 || max_pages > (1u << 30) || max_pages * page_size > (1u << 30))))
+        return fail(APK_DECLINE_SHAPE, "%s: n_seq %zu, max_pages %zu", name, n_seq, max_pages);
+    return APK_OK;
+}
+
+}  // namespace
+
+int apk_attend_paged(apk_ctx* c, const void* q, const void* k_cache, const void* v_cache, size_t capacity, size_t page_size,
+                     const uint32_t* page_table, size_t max_pages, const uint32_t* kv_len, size_t n_seq, size_t n_q, size_t n_kv,
+                     size_t head_dim, float scale, size_t window, void* out, int dtype) {
+    if (!c) return fail(APK_DECLINE_NULL, "apk_attend_paged: ctx is NULL");
+    CallScope s(c);
+    return attend(c, "apk_attend_paged", q, k_cache, v_cache, capacity, page_size, page_table, max_pages, nullptr, kv_len, n_seq,
+                  n_seq, n_q, n_kv, head_dim, scale, window, out, dtype);
+}
+
+int apk_attend_paged_chunk(apk_ctx* c, const void* q, const void* k_cache, const void* v_cache, size_t capacity, size_t page_size,
+                           const uint32_t* page_table, size_t max_pages, const uint32_t* q_off, const uint32_t* kv_len, size_t n_seq,
+                           size_t rows, size_t n_q, size_t n_kv, size_t head_dim, float scale, size_t window, void* out, int dtype) {
+    if (!c) return fail(APK_DECLINE_NULL, "apk_attend_paged_chunk: ctx is NULL");
+    CallScope s(c);
+    if (n_seq && rows && !q_off) return fail(APK_DECLINE_NULL, "apk_attend_paged_chunk: NULL tensor");
+    return attend(c, "apk_attend_paged_chunk", q, k_cache, v_cache, capacity, page_size, page_table, max_pages, q_off, kv_len, n_seq,
+                  rows, n_q, n_kv, head_dim, scale, window, out, dtype);
+}
+
+// header, references, a bit per page, and three arrays of scratch
+size_t apk_pages_words(size_t n_pages) { return 4 + 4 * n_pages + (n_pages + 31) / 32; }
+
+int apk_pages_init(apk_ctx* c, uint32_t* pool, size_t n_pages, size_t page_size, const uint32_t* page_table, size_t max_pages,
+                   const uint32_t* kv_len, size_t n_seq) {
+    if (int rc = pages_check("apk_pages_init", c, pool, n_pages, page_size, page_table, max_pages, kv_len, n_seq)) return rc;
+    CallScope s(c);
+    if (int rc = set_device(c)) return rc;
+    uint32_t n = (uint32_t)n_pages, page = (uint32_t)page_size, mp = (uint32_t)max_pages, ns = (uint32_t)n_seq;
+    void* args[] = {&pool, &n, &page, &page_table, &mp, &kv_len, &ns, &c->fault_dev};
+    return launch(c, "apk_pages_init_k", 1, 1024, 0, args);
+}
+
+int apk_pages_extend(apk_ctx* c, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                     uint32_t* kv_len, size_t n_seq, const uint32_t* n_new, size_t rows, uint32_t* q_off, uint32_t* positions,
+                     uint32_t* slots, uint32_t* pairs, uint32_t* n_pairs) {
+    if (int rc = pages_check("apk_pages_extend", c, pool, n_pages, page_size, page_table, max_pages, kv_len, n_seq)) return rc;
+    CallScope s(c);
+    if (!q_off || !n_pairs || (n_seq && (!n_new || !pairs)) || (rows && (!positions || !slots)))
+        return fail(APK_DECLINE_NULL, "apk_pages_extend: NULL tensor");
+    if (rows > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "apk_pages_extend: too large");
+    if (int rc = set_device(c)) return rc;
+    uint32_t n = (uint32_t)n_pages, page = (uint32_t)page_size, mp = (uint32_t)max_pages, ns = (uint32_t)n_seq, r = (uint32_t)rows;
+    void* args[] = {&pool, &n, &page, &page_table, &mp, &kv_len, &ns, &n_new, &r, &q_off, &positions, &slots, &pairs, &n_pairs, &c->fault_dev};
+    return launch(c, "apk_pages_extend_k", 1, 1024, 0, args);
+}
+
+int apk_pages_fork(apk_ctx* c, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                   uint32_t* kv_len, size_t n_seq, const uint32_t* src, const uint32_t* dst, size_t n) {
+    if (int rc = pages_check("apk_pages_fork", c, pool, n_pages, page_size, page_table, max_pages, kv_len, n_seq)) return rc;
+    CallScope s(c);
+    if (n == 0) return APK_OK;
+    if (!src || !dst) return fail(APK_DECLINE_NULL, "apk_pages_fork: NULL tensor");
+    if (n > 1024 || n_seq == 0) return fail(APK_DECLINE_SHAPE, "apk_pages_fork: %zu pairs (at most 1024), %zu sequences", n, n_seq);
+    if (int rc = set_device(c)) return rc;
+    uint32_t np = (uint32_t)n_pages, page = (uint32_t)page_size, mp = (uint32_t)max_pages, ns = (uint32_t)n_seq, k = (uint32_t)n;
+    void* args[] = {&pool, &np, &page, &page_table, &mp, &kv_len, &ns, &src, &dst, &k, &c->fault_dev};
+    return launch(c, "apk_pages_fork_k", 1, 1024, 0, args);
+}
+
+int apk_pages_truncate(apk_ctx* c, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                       uint32_t* kv_len, size_t n_seq, const uint32_t* new_len) {
+    if (int rc = pages_check("apk_pages_truncate", c, pool, n_pages, page_size, page_table, max_pages, kv_len, n_seq)) return rc;
+    CallScope s(c);
+    if (n_seq == 0) return APK_OK;
+    if (!new_len) return fail(APK_DECLINE_NULL, "apk_pages_truncate: NULL tensor");
+    if (int rc = set_device(c)) return rc;
+    uint32_t n = (uint32_t)n_pages, page = (uint32_t)page_size, mp = (uint32_t)max_pages, ns = (uint32_t)n_seq;
+    void* args[] = {&pool, &n, &page, &page_table, &mp, &kv_len, &ns, &new_len, &c->fault_dev};
+    return launch(c, "apk_pages_truncate_k", 1, 1024, 0, args);
+}
+
+int apk_pages_compact(apk_ctx* c, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                      const uint32_t* kv_len, size_t n_seq, uint32_t* pairs, uint32_t* n_pairs) {
+    if (int rc = pages_check("apk_pages_compact", c, pool, n_pages, page_size, page_table, max_pages, kv_len, n_seq)) return rc;
+    CallScope s(c);
+    if (!n_pairs || (n_pages > 1 && !pairs)) return fail(APK_DECLINE_NULL, "apk_pages_compact: NULL tensor");
+    if (int rc = set_device(c)) return rc;
+    uint32_t n = (uint32_t)n_pages, page = (uint32_t)page_size, mp = (uint32_t)max_pages, ns = (uint32_t)n_seq;
+    void* args[] = {&pool, &n, &page, &page_table, &mp, &kv_len, &ns, &pairs, &n_pairs, &c->fault_dev};
+    return launch(c, "apk_pages_compact_k", 1, 1024, 0, args);
+}
+
+int apk_pages_copy(apk_ctx* c, void* region, size_t n_planes, size_t plane_bytes, size_t n_pages, size_t page_bytes,
+                   const uint32_t* pairs, const uint32_t* n_pairs, size_t max_pairs) {
+    if (!c) return fail(APK_DECLINE_NULL, "apk_pages_copy: ctx is NULL");
+    CallScope s(c);
+    if (n_planes == 0 || n_pages == 0 || max_pairs == 0) return APK_OK;
+    if (!region || !pairs || !n_pairs) return fail(APK_DECLINE_NULL, "apk_pages_copy: NULL tensor");
+    if (!aligned16(region) || page_bytes == 0 || page_bytes % 16 || plane_bytes % 16)
+        return fail(APK_DECLINE_SHAPE, "apk_pages_copy: region, plane_bytes %zu and page_bytes %zu in whole 16-byte tiles", plane_bytes, page_bytes);
+    if (n_pages > 0xffffffffu || n_planes > (1u << 20) || page_bytes > (1ull << 35) || page_bytes > plane_bytes / n_pages || max_pairs > 0x7fffffffu)
+        return fail(APK_DECLINE_SHAPE, "apk_pages_copy: %zu pages of %zu bytes in planes of %zu", n_pages, page_bytes, plane_bytes);
+    if (int rc = set_device(c)) return rc;
+    uint32_t np = (uint32_t)n_pages, npl = (uint32_t)n_planes, mp = (uint32_t)max_pairs;
+    uint64_t plb = plane_bytes, pgb = page_bytes;
+    uint32_t slices = (uint32_t)((page_bytes / 16 + 1023) / 1024);
+    const double items = (double)max_pairs * (double)n_planes * slices;
+    const unsigned grid = items < 4096. ? (unsigned)items : 4096u;
+    void* args[] = {&region, &npl, &plb, &np, &pgb, &pairs, &n_pairs, &mp, &slices, &c->fault_dev};
+    return launch(c, "apk_pages_copy_k", grid, 256, 0, args);
 }
 
 /* ------------------------------------------------------------- launch plans */

@@ -2,9 +2,10 @@
 //
 // Built with `hipcc --genco --offload-arch=gfx950 -ffp-contract=off` into one
 // code object that the host library embeds and loads with hipModuleLoadData.
-// Every kernel here is HBM-bound: wave64, 128-bit global accesses, DPP/shuffle
-// reductions inside a wave, LDS only for cross-wave sums and byte staging.
-// No MFMA: nothing on this path is a contraction.
+// The per-layer ops are HBM-bound: wave64, 128-bit global accesses, DPP/shuffle
+// reductions inside a wave, LDS only for cross-wave sums and byte staging; nothing
+// in them is a contraction.  Attention over the paged cache (attend.hip.h) is one:
+// its products run on the matrix cores.
 //
 // Arithmetic contract (what the CPU reference computes, op for op):
 //   * -ffp-contract=off for the whole file: a*b-c stays two rounded f32 ops,
@@ -25,3 +26,5 @@
 #include "kernels/embed.hip.h"
 #include "kernels/router.hip.h"
 #include "kernels/permute.hip.h"
+#include "kernels/attend.hip.h"
+#include "kernels/pages.hip.h"

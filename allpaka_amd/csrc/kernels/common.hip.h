@@ -14,7 +14,8 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 #define APK_FAULT_TOKEN_RANGE 1u   // embedding id >= vocab
 #define APK_FAULT_EXPERT_RANGE 2u  // routed expert id >= n_expert
 #define APK_FAULT_ROW_RANGE 4u     // gather index >= source rows
-#define APK_FAULT_CACHE_RANGE 8u   // KV-cache position >= capacity
+#define APK_FAULT_CACHE_RANGE 8u   // KV-cache position >= capacity, or a page table that does not name pages of the cache
+#define APK_FAULT_NO_PAGES 16u     // fewer free pages than a step needs
 
 DEV float h2f(uint32_t bits16) { return (float)__builtin_bit_cast(f16_t, (uint16_t)bits16); }
 

@@ -10,6 +10,7 @@ F32, F16 = 0, 1
 FMT_Q4K, FMT_Q5K, FMT_Q6K, FMT_Q8_0, FMT_Q2K, FMT_Q3K, FMT_Q5_0, FMT_F16, FMT_F32, FMT_BF16 = range(10)
 DECLINE_UNSUPPORTED, DECLINE_SHAPE, DECLINE_NULL, DECLINE_RANGE, DECLINE_NO_DEVICE, DECLINE_NOT_ATTACHED, DECLINE_CAPTURE = range(1, 8)
 FAULT_TOKEN_RANGE, FAULT_EXPERT_RANGE, FAULT_ROW_RANGE, FAULT_CACHE_RANGE = 1, 2, 4, 8
+FAULT_NO_PAGES = 16
 
 
 
@@ -96,6 +97,15 @@ SYMBOLS = {
     "apk_cast": (_i, [_vp, _vp, _i, _vp, _i, _sz]),
     "apk_moe_shared_hits": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp]),
     "apk_attn_prologue_rows": (_i, [_vp, C.POINTER(AttnPrologue)]),
+    "apk_attend_paged": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _f, _sz, _vp, _i]),
+    "apk_attend_paged_chunk": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _f, _sz, _vp, _i]),
+    "apk_pages_words": (_sz, [_sz]),
+    "apk_pages_init": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz]),
+    "apk_pages_extend": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp]),
+    "apk_pages_fork": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz]),
+    "apk_pages_truncate": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp]),
+    "apk_pages_compact": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "apk_pages_copy": (_i, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _sz]),
     "apk_plan_embed_rows": (_i, [_i, _sz, _sz, _i, _plan]),
     "apk_kernel_count": (_sz, []),
     "apk_kernel_name": (_i, [_sz, C.c_char_p, _sz]),

@@ -81,7 +81,8 @@ enum apk_fault {
     APK_FAULT_TOKEN_RANGE = 1,  /* an embedding id >= vocab was met on the device  */
     APK_FAULT_EXPERT_RANGE = 2, /* a routed expert id >= n_expert                  */
     APK_FAULT_ROW_RANGE = 4,    /* a gather / scatter row index out of range       */
-    APK_FAULT_CACHE_RANGE = 8   /* a KV-cache position >= capacity                 */
+    APK_FAULT_CACHE_RANGE = 8,  /* a KV-cache position >= capacity; a page table that does not name pages of its cache */
+    APK_FAULT_NO_PAGES = 16     /* apk_pages_extend: fewer free pages than the step needs */
 };
 
 /* ------------------------------------------------------------ life cycle ---- */
@@ -438,6 +439,95 @@ int apk_argmax_rows(apk_ctx* ctx, const float* logits, size_t rows, size_t n, ui
  * (APK_DECLINE_SHAPE).  May be recorded (apk_capture_begin .. _end).  Every call on a GPU shares that GPU's array:
  * calls that overlap on one GPU -- two contexts, or one context from two host threads without its lock -- race. */
 int apk_argmax_rows_noalloc(apk_ctx* ctx, const float* logits, size_t rows, size_t n, uint32_t* out);
+
+/* ------------------------------------------------------- the paged cache ---- */
+
+/* Many sequences in one K/V cache.  A plane (one layer's K or V) is fp16 [capacity][n_kv*head_dim], the planes that
+ * apk_qknorm_rope_kv_store and apk_attn_prologue_rows write; page p of it is the rows [p*page_size, (p+1)*page_size).
+ * Key j of sequence s is cache row page_table[s][j / page_size] * page_size + j % page_size in every plane.
+ * page_table: u32[n_seq][max_pages]; kv_len: u32[n_seq], the tokens a sequence holds; entries that no token needs may
+ * hold anything, and so may cache rows that no sequence holds (NaN included): they are not read, or not used.  A flat
+ * cache of one session is a table of one entry, 0, and page_size = capacity.  Any page_size >= 1;
+ * max_pages * page_size <= 2^30; capacity < 2^32.  No counterpart in the reference, whose caches are flat (kv.rs). */
+
+/* Attention of ONE new token per sequence over the paged cache: with p = kv_len[s] - 1 (the token's own K and V are in
+ * the cache already), head h of row s, and kv head g = h / (n_q / n_kv),
+ *   x_j = scale * <q[s][h], K[row of j][g]>  for max(0, p - window + 1) <= j <= p   (window 0: all j <= p),
+ *   out[s][h] = sum_j exp(x_j - max x) V[row of j][g] / sum_j exp(x_j - max x);   zeros for a row that sees no key.
+ * The step between the K/V store and the output projection that gpu::attend / attn_block of the reference's surface
+ * stand for (gpu/stub.rs; scale and window of AttnBlockReq, gpu/types.rs:302-365).
+ * q, out: [n_seq][n_q*head_dim] of dtype (out may be q); k_cache, v_cache: one layer's planes; n_q a multiple of n_kv.
+ * The products take all bits of fp16 and f32 queries (an f32 as the sum of two fp16), sums are f32; probabilities are
+ * rounded to fp16 for fp16 rows and keep 22 bits for f32 rows.  Heads of 64, 128 and 256 run on the matrix cores; other
+ * sizes up to 1024 element by element (right, and slow).  K or V rows that a row sees and that hold infinities or NaN
+ * make its result infinite or NaN, in V the channels concerned; those it does not see do not reach it.
+ * kv_len[s] > max_pages * page_size is cut to it, a table entry >= capacity / page_size that is needed reads page 0;
+ * both raise APK_FAULT_CACHE_RANGE, and the rows of that sequence are then unspecified.
+ * Uses a scratch of the context (256 MiB, allocated by the first call that may need it: inside a recording that call is
+ * declined with APK_DECLINE_CAPTURE, run the step once unrecorded first).  May be recorded. */
+int apk_attend_paged(apk_ctx* ctx, const void* q, const void* k_cache, const void* v_cache, size_t capacity, size_t page_size,
+                     const uint32_t* page_table, size_t max_pages, const uint32_t* kv_len, size_t n_seq, size_t n_q,
+                     size_t n_kv, size_t head_dim, float scale, size_t window, void* out, int dtype);
+
+/* The same for chunks: sequence s brings the rows q_off[s] .. q_off[s+1] (u32[n_seq+1], ascending, on the device; any
+ * number of rows, none included), whose K and V are in the cache already: row i of m is at position kv_len[s] - m + i and
+ * sees no later key (a position below 0: zeros).  Prompts, chunks of prompts over what is cached, drafts to verify, single
+ * tokens, mixed in one call.  q, out: [rows][n_q*head_dim]; rows at and behind q_off[n_seq] are left as they are; a row
+ * index > rows or a descending pair raises APK_FAULT_ROW_RANGE and is cut off.  The reference's gpu::attend_batch and the
+ * attention of PrefillAttnReq (gpu/stub.rs, gpu/types.rs:302-365). */
+int apk_attend_paged_chunk(apk_ctx* ctx, const void* q, const void* k_cache, const void* v_cache, size_t capacity,
+                           size_t page_size, const uint32_t* page_table, size_t max_pages, const uint32_t* q_off,
+                           const uint32_t* kv_len, size_t n_seq, size_t rows, size_t n_q, size_t n_kv, size_t head_dim,
+                           float scale, size_t window, void* out, int dtype);
+
+/* Who holds which page.  The state is three device arrays of the caller's: pool (u32[apk_pages_words(n_pages)]: the number
+ * of free pages in word 0, the holders of page p in word 4 + p, then what the library keeps), page_table and kv_len as
+ * above.  The entries below change them on the device in stream order, so a recorded step can be replayed for every
+ * token; what they choose follows from the state alone.  One pool belongs to one page_table of n_seq sequences; a sequence
+ * without tokens holds nothing. */
+size_t apk_pages_words(size_t n_pages);
+
+/* Counts the pool afresh from page_table and kv_len (n_seq 0: every page is free).  An entry >= n_pages or a length past
+ * the table raises APK_FAULT_CACHE_RANGE and is left out. */
+int apk_pages_init(apk_ctx* ctx, uint32_t* pool, size_t n_pages, size_t page_size, const uint32_t* page_table,
+                   size_t max_pages, const uint32_t* kv_len, size_t n_seq);
+
+/* n_new[s] more tokens for every sequence (0: none): pages are taken as they are needed, the lowest free ones first,
+ * sequences in order.  A sequence about to write into a page that others hold as well gets a copy of it first (of holders
+ * that all write in this call the last keeps the page): pairs [n_seq][2] = (copy, original), *n_pairs of them in order,
+ * for apk_pages_copy, which has to run before anything is stored.  Then kv_len[s] += n_new[s], and for the new rows,
+ * sequence after sequence: q_off u32[n_seq+1]; positions u32[rows] (for apk_rope_table); slots u32[rows], their cache rows
+ * (cache_pos of apk_qknorm_rope_kv_store and apk_attn_prologue_rows); rows of nobody get position 0 and slot 2^32 - 1,
+ * which those entries skip (and report).  All or nothing: with too few free pages (APK_FAULT_NO_PAGES), more new tokens
+ * than rows (APK_FAULT_ROW_RANGE), a sequence that would not fit its table or whose table names no page
+ * (APK_FAULT_CACHE_RANGE) nothing changes, q_off and *n_pairs are 0 and every row is nobody's. */
+int apk_pages_extend(apk_ctx* ctx, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                     uint32_t* kv_len, size_t n_seq, const uint32_t* n_new, size_t rows, uint32_t* q_off,
+                     uint32_t* positions, uint32_t* slots, uint32_t* pairs, uint32_t* n_pairs);
+
+/* Sequence dst[i], which must hold nothing, becomes a further holder of all pages of sequence src[i], for i < n <= 1024 (beam
+ * search, several answers to one prompt): no cache row is copied.  All as the tables are when the call begins.  A pair
+ * that names no sequence, the same one twice, a dst that holds something or that an earlier pair named is left out and
+ * raises APK_FAULT_ROW_RANGE. */
+int apk_pages_fork(apk_ctx* ctx, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                   uint32_t* kv_len, size_t n_seq, const uint32_t* src, const uint32_t* dst, size_t n);
+
+/* Cuts sequences to new_len[s] tokens (drafts that were not accepted); 0 frees a sequence, a length that is not below
+ * kv_len[s] leaves it.  Pages that nobody holds any more are free. */
+int apk_pages_truncate(apk_ctx* ctx, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                       uint32_t* kv_len, size_t n_seq, const uint32_t* new_len);
+
+/* Moves the pages in use to the front: with L of them, the i-th of those at or behind L goes to the i-th free one before it.
+ * Renames them in pool and page_table and lists the moves in pairs [n_pages / 2][2], *n_pairs of them, for
+ * apk_pages_copy, which has to run before the cache is read again. */
+int apk_pages_compact(apk_ctx* ctx, uint32_t* pool, size_t n_pages, size_t page_size, uint32_t* page_table, size_t max_pages,
+                      const uint32_t* kv_len, size_t n_seq, uint32_t* pairs, uint32_t* n_pairs);
+
+/* In each of n_planes planes (plane i at region + i * plane_bytes): page pairs[j][1] copied over page pairs[j][0], for
+ * j < min(*n_pairs, max_pairs); pairs and n_pairs on the device, as the entries above write them (no page is both a copy
+ * and an original).  page_bytes: page_size * n_kv * head_dim * 2; it and plane_bytes multiples of 16. */
+int apk_pages_copy(apk_ctx* ctx, void* region, size_t n_planes, size_t plane_bytes, size_t n_pages, size_t page_bytes,
+                   const uint32_t* pairs, const uint32_t* n_pairs, size_t max_pairs);
 
 /* dst = src, `bytes` a multiple of 16: the plain stream kernel the bandwidth
  * figures of the other kernels are calibrated against. */
