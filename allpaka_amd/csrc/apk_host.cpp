@@ -78,10 +78,11 @@ std::vector<std::string> all_kernel_names() {
                                   "apk_pages_init_k", "apk_pages_extend_k", "apk_pages_fork_k", "apk_pages_truncate_k", "apk_pages_compact_k", "apk_pages_copy_k"};
     for (const char* t : {"f32", "f16"}) {
         for (int hd : kAttendHeadDims) {
-            v.push_back(std::string("apk_attend_token_") + t + "_hd" + std::to_string(hd) + "_w4");
+            for (int nb : {1, 2, 4})
+                if (hd * nb <= 512) v.push_back(std::string("apk_attend_few_") + t + "_hd" + std::to_string(hd) + "_b" + std::to_string(nb));
             v.push_back(std::string("apk_attend_chunk_") + t + "_hd" + std::to_string(hd));
         }
-        for (const char* w : {"_w1", "_w4"}) v.push_back(std::string("apk_attend_join_") + t + w);
+        v.push_back(std::string("apk_attend_join_") + t);
         v.push_back(std::string("apk_attend_any_") + t);
         for (const char* f : {"q5k", "q6k", "q2k", "q3k", "q5_0", "f16", "f32", "bf16"}) v.push_back(std::string("apk_embed_") + f + "_" + t);
         for (int c : kAddnormTiles) v.push_back(std::string("apk_add_rmsnorm_") + t + "_c" + std::to_string(c));
@@ -1580,6 +1581,10 @@ int apk_argmax_rows(apk_ctx* c, const float* logits, size_t rows, size_t n, uint
 namespace {
 
 const size_t kAttendScratch = 256u << 20;
+#ifndef V_TT
+#define V_TT 256
+#define V_UM 2
+#endif
 
 // page / key arithmetic of the kernels: floor(2^32 / page), 2^32 - 1 for page 1
 uint32_t page_magic(size_t page) { return page == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / page); }
@@ -1598,7 +1603,7 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
     if (max_pages == 0 || max_pages > (1u << 30) || page_size > (1u << 30) || max_pages * page_size > (1u << 30))
         return fail(APK_DECLINE_SHAPE, "%s: max_pages %zu * page_size %zu (1..2^30)", name, max_pages, page_size);
     if (n_seq == 0 || rows == 0) return APK_OK;
-    if (n_seq > 0x7fffffffu || rows > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
+    if (n_seq > 0x7fffffffu || rows > 0x7fffffffu / (n_q / n_kv)) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
     if (!q || !k_cache || !v_cache || !page_table || !kv_len || !out) return fail(APK_DECLINE_NULL, "%s: NULL tensor", name);
     if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
         return fail(APK_DECLINE_SHAPE, "%s: tensors must be 16-byte aligned", name);
@@ -1625,58 +1630,87 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
     a.window = window >= max_pages * page_size ? 0 : (uint32_t)window;
     a.c = fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f);  // above zero: a masked score stays -inf when multiplied by it
     a.sign = scale < 0.f ? -1.f : 1.f;
-    a.head_tiles = 1;
-    const std::string t = dtype == APK_F32 ? "f32" : "f16";
+    const std::string t_name = dtype == APK_F32 ? "f32" : "f16";
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
         if (rows * n_q > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
+        a.tile_rows = 1;
+        a.unit = 1;
         if (int rc = set_device(c)) return rc;
         void* args[] = {&a};
-        return launch(c, "apk_attend_any_" + t, (unsigned)(rows * n_q), 256, (unsigned)((5 * head_dim + 8) * 4), args);
+        return launch(c, "apk_attend_any_" + t_name, (unsigned)(rows * n_q), 256, (unsigned)((5 * head_dim + 8) * 4), args);
     }
-    unsigned shmem;
-    uint64_t tiles;
+    // Tiles of few rows (16, 32 or 64, whichever holds the rows of a sequence on average) read the cache straight into
+    // registers; more rows share it through LDS in tiles of 128.  (Heads of 256: 64 rows would not leave registers.)
+    unsigned shmem, block;
     std::string kernel;
-    if (!q_off) {
-        a.tile_rows = APK_ATT_TOKEN_ROWS;
-        a.unit = APK_ATT_TOKEN_UNIT;
-        a.head_tiles = (a.group + APK_ATT_TOKEN_ROWS - 1) / APK_ATT_TOKEN_ROWS;
-        a.target = 1024;
-        a.unit_min = 2;
-        tiles = n_seq;
-        const unsigned r = a.group < APK_ATT_TOKEN_ROWS ? a.group : APK_ATT_TOKEN_ROWS;
-        shmem = (unsigned)((2 * 4 * 16 + 4 * r * head_dim) * 4);
-        kernel = "apk_attend_token_" + t + "_hd" + std::to_string(head_dim) + "_w4";
+    const double flat = (double)rows * a.group / (double)n_seq;  // rows of a kv head per sequence
+    #ifndef V_NB1
+#define V_NB1 8.
+#define V_NB2 16.
+#endif
+    const unsigned nb = !q_off || flat <= V_NB1 ? 1 : flat <= V_NB2 ? 2 : flat <= 64. && head_dim < 256 ? 4 : 0;
+    if (nb) {
+        const unsigned waves = head_dim == 256 || (head_dim == 128 && nb == 4) ? 4 : 8;
+        a.tile_rows = 16 * nb;
+        a.unit = 32;
+        a.heads = 1;
+        while (a.heads < waves && n_kv % (2 * a.heads) == 0) a.heads *= 2;
+        a.unit_min = V_UM;
+        const unsigned r = !q_off && a.group < a.tile_rows ? a.group : a.tile_rows;
+        block = waves * 64;
+        shmem = a.heads == waves ? 0 : (unsigned)((2 * waves * a.tile_rows + waves * r * head_dim) * 4);
+        kernel = "apk_attend_few_" + t_name + "_hd" + std::to_string(head_dim) + "_b" + std::to_string(nb);
     } else {
         a.tile_rows = APK_ATT_CHUNK_ROWS;
-        a.unit = head_dim == 256 ? 32 : APK_ATT_CHUNK_UNIT;
+        a.unit = head_dim == 256 ? 32 : 64;
+        a.heads = 1;
         a.target = 512;
         a.unit_min = 512 / a.unit;
-        tiles = rows * (uint64_t)a.group / APK_ATT_CHUNK_ROWS + n_seq;
+        block = 256;
         shmem = (unsigned)(4 * a.unit * head_dim * 2);
-        kernel = "apk_attend_chunk_" + t + "_hd" + std::to_string(head_dim);
+        kernel = "apk_attend_chunk_" + t_name + "_hd" + std::to_string(head_dim);
     }
-    // slots never exceed 2 * target: a cut tile has at least two parts, of more than half of a part's share of all units
-    const size_t slot = (size_t)a.tile_rows * (head_dim + 2) * 4;
-    if (2 * (size_t)a.target * slot > kAttendScratch) a.target = (uint32_t)(kAttendScratch / (2 * slot));
-    const uint64_t H = (uint64_t)n_kv * a.head_tiles;
-    const uint64_t units = (max_pages * page_size + a.unit - 1) / a.unit;
-    const uint64_t parts = units > a.unit_min ? (units + a.unit_min - 1) / a.unit_min : 1;  // of a tile at most
-    uint64_t items = tiles + (a.target + H - 1) / H + 1;
-    if (parts < items && tiles * parts < items) items = tiles * parts;
-    if (items * H > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
+    const uint64_t tiles = rows * (uint64_t)a.group / a.tile_rows + n_seq, hblocks = n_kv / a.heads;
+    const uint64_t units = (max_pages * page_size + a.unit - 1) / a.unit;  // of a tile at most
+    const size_t fit = (kAttendScratch - APK_ATT_PART_AT) / (2 * (size_t)a.tile_rows * (head_dim + 2) * 4);  // pairs of slots
+    uint64_t items, listed;
+    bool cut;
+    if (nb) {
+        // as many workgroups as fill the chip, each with at most two cut segments
+        uint64_t t = (V_TT + hblocks - 1) / hblocks;
+        if (t * n_kv > fit) t = fit / n_kv;
+        if (t > APK_ATT_MAX_LIST) t = APK_ATT_MAX_LIST;
+        if (tiles * units < t * a.unit_min) t = (tiles * units + a.unit_min - 1) / a.unit_min;
+        if (t == 0) return fail(APK_DECLINE_SHAPE, "%s: n_kv %zu", name, n_kv);
+        a.target = (uint32_t)t;
+        a.list_tiles = tiles <= t;
+        a.join_rows = tiles * 32 < t ? 1 : 8;
+        items = t;
+        listed = a.list_tiles ? tiles : t;
+        cut = units > 1 && t > 1;
+    } else {
+        // A cut tile has at least two parts, of more than half of a part's share of all units: no more than 2 * target
+        // parts come of cutting, of no more than target tiles.
+        if (a.target > fit) a.target = (uint32_t)fit;
+        const uint64_t parts = units > a.unit_min ? (units + a.unit_min - 1) / a.unit_min : 1;
+        items = tiles + (a.target + hblocks - 1) / hblocks + 1;
+        if (tiles * parts < items) items = tiles * parts;
+        listed = (a.target + hblocks - 1) / hblocks;
+        if (tiles < listed) listed = tiles;
+        a.join_rows = 8;
+        cut = parts > 1;
+    }
+    if (items * hblocks > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);
     if (int rc = set_device(c)) return rc;
-    if (parts > 1 && !c->attend_part) {
+    if (cut && !c->attend_part) {
         if (c->capturing) return fail(APK_DECLINE_CAPTURE, "%s: the scratch would have to be allocated inside a recording (run once unrecorded first)", name);
         HIP_TRY(hipMalloc(&c->attend_part, kAttendScratch));
     }
-    a.part = (float*)c->attend_part;
+    a.scratch = cut ? (uint32_t*)c->attend_part : nullptr;
     void* args[] = {&a};
-    if (int rc = launch(c, kernel, (unsigned)(items * H), 256, shmem, args)) return rc;
-    if (parts == 1) return APK_OK;
-    uint64_t cut = tiles * H < a.target ? tiles * H : a.target;  // tiles that may have been cut
-    cut = (cut + H - 1) / H * H;
-    if (q_off) return launch(c, "apk_attend_join_" + t + "_w1", (unsigned)(cut * (a.tile_rows / 4)), 256, 0, args);
-    return launch(c, "apk_attend_join_" + t + "_w4", (unsigned)(cut * a.tile_rows), 256, 0, args);
+    if (int rc = launch(c, kernel, (unsigned)(items * hblocks), block, shmem, args)) return rc;
+    if (!cut) return APK_OK;
+    return launch(c, "apk_attend_join_" + t_name, (unsigned)(listed * n_kv * (a.tile_rows / a.join_rows)), 512, 0, args);
 }
 
 // The checks that the page entries share.

@@ -54,102 +54,96 @@ DEV void split_key(const apk_attend_args& a, uint32_t key, uint32_t& idx, uint32
 }
 
 // ------------------------------------------------------------------------------------------- division of the work
-// A tile is tile_rows flat rows (token * group + head of the group) of one sequence and kv head.  Every sequence's tiles
-// are cut into the same number of parts along the keys: one, where there are tiles enough to fill the chip, else as many
-// as bring the launch to about `target` workgroups, parts of at least unit_min units.  The lengths are on the device, so
-// each workgroup works its own place out: two short passes of a wave over the sequences.
+// A tile is tile_rows flat rows (token * group + head of the group) of one sequence and kv head, its work the units of keys
+// that its rows see.  The lengths are on the device, so each workgroup works its own place out: two short passes of a wave
+// over the sequences (sums and prefix sums by DPP).  The tiles that were cut are listed in the scratch for the launch that
+// joins their parts.
+// Chunks (att_find): a workgroup per tile, the heaviest first; where there are too few tiles to fill the chip, the tiles of
+// a sequence are cut into as many parts as bring the launch to about `target` workgroups, of at least unit_min units.
+// Few rows (att_share): all units in one line, cut into `target` equal pieces, one for each workgroup, which goes through
+// the tiles its piece touches.  Such launches are streams of the cache: equal pieces end together whatever the lengths are.
 struct att_seq {
     uint32_t row0, m;  // first row, rows
     int32_t n, p0;     // keys, position of the first row
-    uint32_t tiles, parts, umax;
+    uint32_t tiles, umax, parts;
 };
 struct att_item {
-    uint32_t seq, tile, part, slot;
+    uint32_t seq, tile, part, slot;  // slot: of this part, among all parts of cut tiles
     att_seq s;
 };
 DEV att_seq att_load_seq(const apk_attend_args& a, uint32_t i) {
-    att_seq s;
+    att_seq s = {0, 0, 0, 0, 0, 0, 1};
+    if (i >= a.n_seq) return s;
     uint32_t n = a.kv_len[i];
-    const uint64_t cap = (uint64_t)a.max_pages * a.page;
-    bool bad = n > cap;
-    if (bad) n = (uint32_t)cap;
-    uint32_t r0 = i, r1 = i + 1;
+    uint32_t r0 = i, r1 = i + 1, bad = 0;
     if (a.q_off) {
         r0 = a.q_off[i];
         r1 = a.q_off[i + 1];
         if (r1 > a.rows || r0 > r1) {
-            atomicOr(a.fault, APK_FAULT_ROW_RANGE);
+            bad = APK_FAULT_ROW_RANGE;
             r1 = r1 < a.rows ? r1 : a.rows;
             r0 = r0 < r1 ? r0 : r1;
         }
     }
-    if (bad) atomicOr(a.fault, APK_FAULT_CACHE_RANGE);
+    const uint32_t cap = a.max_pages * a.page;  // at most 2^30
+    if (n > cap) {
+        n = cap;
+        bad |= APK_FAULT_CACHE_RANGE;
+    }
+    if (bad) atomicOr(a.fault, bad);
     s.row0 = r0;
     s.m = r1 - r0;
     s.n = (int32_t)n;
     s.p0 = (int32_t)n - (int32_t)s.m;
-    const uint64_t flat = (uint64_t)s.m * a.group;
-    s.tiles = a.q_off ? (uint32_t)((flat + a.tile_rows - 1) / a.tile_rows) : (s.m ? 1u : 0u);
+    s.tiles = (uint32_t)(((uint64_t)s.m * a.group + a.tile_rows - 1) / a.tile_rows);
     uint32_t span = n;
     if (a.window) {  // keys that the rows of one tile see between them
-        const uint64_t w = (uint64_t)a.window + (a.q_off ? a.tile_rows / a.group + 1 : 0) + a.unit;
+        const uint64_t w = (uint64_t)a.window + a.tile_rows / a.group + 1 + a.unit;
         if (w < span) span = (uint32_t)w;
     }
     s.umax = (span + a.unit - 1) / a.unit;
-    s.parts = 1;
+    if (s.umax == 0) s.umax = 1;  // rows without keys are work too: they get zeros
     return s;
 }
 DEV uint32_t rl(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
-DEV uint64_t rl64(uint64_t v, int lane) { return ((uint64_t)rl((uint32_t)(v >> 32), lane) << 32) | rl((uint32_t)v, lane); }
-DEV uint64_t wave_scan_u64(uint64_t v) {  // inclusive sums over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t t = ((uint64_t)(uint32_t)__shfl_up((uint32_t)(v >> 32), d) << 32) | (uint32_t)__shfl_up((uint32_t)v, d);
-        if ((int)(threadIdx.x & 63) >= d) v += t;
-    }
+template <int CTRL, int ROWS> DEV uint32_t dpp_add(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);
+}
+DEV uint32_t wave_scan_u32(uint32_t v) {  // inclusive sums over the lanes
+    v = dpp_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast 15, 31
+    v = dpp_add<0x143, 0xc>(v);
     return v;
 }
-DEV uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t lo = __shfl_xor((uint32_t)v, d), hi = __shfl_xor((uint32_t)(v >> 32), d);
-        v += ((uint64_t)hi << 32) | lo;
-    }
-    return v;
-}
-// Units a part has at least, so that no more than `target` parts come of splitting.
-DEV uint32_t att_units_per_part(const apk_attend_args& a) {
+// Units a part has at least, so that at most `target` workgroups' worth of parts comes of cutting.  (Sums of whole numbers
+// in double: exact, and the same in every wave.)
+DEV uint32_t att_units_per_part(const apk_attend_args& a, const att_seq& first) {
     const uint32_t lane = threadIdx.x & 63;
-    uint64_t u = 0;
-    for (uint32_t i = lane; i < a.n_seq; i += 64) {
+    double u = (double)first.tiles * (double)first.umax;
+    for (uint32_t i = 64 + lane; i < a.n_seq; i += 64) {
         const att_seq s = att_load_seq(a, i);
-        u += (uint64_t)s.tiles * s.umax;
+        u += (double)s.tiles * (double)s.umax;
     }
-    u = (a.n_seq > 1 ? wave_sum_u64(u) : rl64(u, 0)) * a.n_kv * a.head_tiles;
-    const uint64_t c = (u + a.target - 1) / a.target;
-    return c > a.unit_min ? (uint32_t)c : a.unit_min;
+    u = group_sum<64>(u) * (double)(a.n_kv / a.heads);
+    const double c = ceil(u / (double)a.target);
+    return c > (double)a.unit_min ? (c < 1073741824.0 ? (uint32_t)c : 1073741824u) : a.unit_min;
 }
 DEV uint32_t att_parts(const att_seq& s, uint32_t c) { return s.umax > c ? (s.umax + c - 1) / c : 1u; }
-// The tile and part that item `pg` (0, 1, ...; without the kv head) of the launch is; false: past the last one.  SPLIT:
-// items are the tiles that were cut, `slot` the first of a tile's parts.
-template <bool SPLIT> DEV bool att_find(const apk_attend_args& a, uint32_t pg, att_item& it) {
-    const uint32_t lane = threadIdx.x & 63, c = att_units_per_part(a);
-    uint64_t before = 0, slots = 0;
-    for (uint32_t base = 0; base < a.n_seq; base += 64) {
-        const uint32_t i = base + lane;
-        att_seq s = {0, 0, 0, 0, 0, 1, 0};
-        if (i < a.n_seq) {
-            s = att_load_seq(a, i);
-            s.parts = att_parts(s, c);
-        }
-        const uint64_t parts = (uint64_t)s.tiles * s.parts, cut = s.parts > 1 ? parts : 0;
-        const uint64_t cnt = SPLIT ? (s.parts > 1 ? s.tiles : 0) : parts;
-        uint64_t inc = cnt, sinc = cut;
-        if (a.n_seq > 1) {
-            inc = wave_scan_u64(inc);
-            sinc = wave_scan_u64(sinc);
-        }
-        const uint64_t hit = __ballot(before + inc > pg && before + inc - cnt <= pg);
+// The tile and part that item `pg` (0, 1, ...; without the kv heads) of the launch is; false: past the last one.
+DEV bool att_find(const apk_attend_args& a, uint32_t pg, att_item& it) {
+    const uint32_t lane = threadIdx.x & 63;
+    att_seq s = att_load_seq(a, lane);
+    const uint32_t c = att_units_per_part(a, s);
+    uint32_t before = 0, slots = 0, tiles = 0;
+    bool found = false;
+    for (uint32_t base = 0;;) {
+        s.parts = att_parts(s, c);
+        const uint32_t cnt = s.tiles * s.parts, cut = s.parts > 1 ? cnt : 0, ct = s.parts > 1 ? s.tiles : 0;
+        const uint32_t inc = before + wave_scan_u32(cnt), sinc = slots + wave_scan_u32(cut), tinc = tiles + wave_scan_u32(ct);
+        const uint64_t hit = __ballot(inc > pg && inc - cnt <= pg);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             it.seq = base + (uint32_t)l;
@@ -160,20 +154,101 @@ template <bool SPLIT> DEV bool att_find(const apk_attend_args& a, uint32_t pg, a
             it.s.tiles = rl(s.tiles, l);
             it.s.parts = rl(s.parts, l);
             it.s.umax = rl(s.umax, l);
-            const uint32_t idx = pg - (uint32_t)(before + rl64(inc - cnt, l));
-            const uint32_t slot0 = (uint32_t)(slots + rl64(sinc - cut, l));
-            it.tile = it.s.tiles - 1 - (SPLIT ? idx : idx / it.s.parts);  // the last rows see the most keys: they go first
-            it.part = SPLIT ? 0 : idx % it.s.parts;
-            it.slot = slot0 + (SPLIT ? idx * it.s.parts : idx);
-            return true;
+            const uint32_t idx = pg - rl(inc - cnt, l), rank = idx / it.s.parts;
+            it.tile = it.s.tiles - 1 - rank;  // the last rows see the most keys: they go first
+            it.part = idx - rank * it.s.parts;
+            it.slot = rl(sinc - cut, l) + idx;
+            found = true;
+            const uint32_t at = rl(tinc - ct, l) + rank;  // (lanes are read where all of them are active)
+            if (it.s.parts > 1 && it.part == 0 && threadIdx.x == 0 && blockIdx.x % (a.n_kv / a.heads) == 0) {
+                uint32_t* d = a.scratch + 16 + 8 * at;
+                *(u32x4*)d = u32x4{it.s.row0, it.s.m, it.tile, it.s.parts};
+                *(u32x4*)(d + 4) = u32x4{it.slot, it.slot + 1, 1, 0};
+            }
+            if (blockIdx.x) return true;  // the first workgroup goes on to the number of cut tiles
         }
-        if (a.n_seq > 64) {
-            before += rl64(inc, 63);
-            slots += rl64(sinc, 63);
+        base += 64;
+        before = rl(inc, 63);
+        slots = rl(sinc, 63);
+        tiles = rl(tinc, 63);
+        if (base >= a.n_seq) {
+            if (blockIdx.x == 0 && threadIdx.x == 0 && a.scratch) a.scratch[0] = tiles;
+            return found;
         }
+        s = att_load_seq(a, base + lane);
     }
-    return false;
 }
+DEV uint64_t rl64(uint64_t v, int lane) { return ((uint64_t)rl((uint32_t)(v >> 32), lane) << 32) | rl((uint32_t)v, lane); }
+template <int CTRL, int ROWS> DEV uint64_t dpp_add64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, true);
+    return v + (((uint64_t)hi << 32) | lo);
+}
+DEV uint64_t wave_scan_u64(uint64_t v) {
+    v = dpp_add64<0x111, 0xf>(v);
+    v = dpp_add64<0x112, 0xf>(v);
+    v = dpp_add64<0x114, 0xf>(v);
+    v = dpp_add64<0x118, 0xf>(v);
+    v = dpp_add64<0x142, 0xa>(v);
+    v = dpp_add64<0x143, 0xc>(v);
+    return v;
+}
+// The piece [x0, x1) of the line of all units that workgroup w of `target` takes; empty for workgroups that are not needed.
+// Returns the number of tiles.
+DEV uint32_t att_share(const apk_attend_args& a, uint32_t w, uint64_t& x0, uint64_t& x1, uint64_t& share) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint64_t all = 0;
+    uint32_t tiles = 0;
+    for (uint32_t base = 0; base < a.n_seq; base += 64) {
+        const att_seq s = att_load_seq(a, base + lane);
+        all += rl64(wave_scan_u64((uint64_t)s.tiles * s.umax), 63);
+        tiles += rl(wave_scan_u32(s.tiles), 63);
+    }
+    share = (all + a.target - 1) / a.target;
+    if (share < a.unit_min) share = a.unit_min;
+    x0 = min(all, share * w);
+    x1 = min(all, x0 + share);
+    return tiles;
+}
+// The tile that unit x of the line falls into, where its units begin, and its number among all tiles.
+struct att_place {
+    uint32_t seq, tile, number;
+    uint64_t begin;
+    att_seq s;
+};
+DEV void att_locate(const apk_attend_args& a, uint64_t x, att_place& pl) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint64_t before = 0;
+    uint32_t tiles = 0;
+    for (uint32_t base = 0; base < a.n_seq; base += 64) {
+        const att_seq s = att_load_seq(a, base + lane);
+        const uint64_t cnt = (uint64_t)s.tiles * s.umax, inc = before + wave_scan_u64(cnt);
+        const uint32_t tinc = tiles + wave_scan_u32(s.tiles);
+        const uint64_t hit = __ballot(inc > x && inc - cnt <= x);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            pl.seq = base + (uint32_t)l;
+            pl.s.row0 = rl(s.row0, l);
+            pl.s.m = rl(s.m, l);
+            pl.s.n = (int32_t)rl((uint32_t)s.n, l);
+            pl.s.p0 = (int32_t)rl((uint32_t)s.p0, l);
+            pl.s.tiles = rl(s.tiles, l);
+            pl.s.umax = rl(s.umax, l);
+            pl.s.parts = 1;
+            const uint64_t first = rl64(inc - cnt, l);
+            pl.tile = (uint32_t)((x - first) / pl.s.umax);
+            pl.number = rl(tinc - s.tiles, l) + pl.tile;
+            pl.begin = first + (uint64_t)pl.tile * pl.s.umax;
+            return;
+        }
+        before = rl64(inc, 63);
+        tiles = rl(tinc, 63);
+    }
+}
+DEV float* att_part(const apk_attend_args& a, uint32_t slot, uint32_t kvh) {
+    return (float*)((char*)a.scratch + APK_ATT_PART_AT) + ((uint64_t)slot * a.n_kv + kvh) * ((uint64_t)a.tile_rows * (a.hd + 2));
+}
+DEV float att_inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }  // no key: zeros; NaN stays
 
 // The keys [lo, hi) that any row of a tile sees (tok0 .. tok1: its first and last row of the sequence) and, of their
 // units, those of one part.
@@ -195,18 +270,25 @@ DEV att_span att_tile_span(const apk_attend_args& a, const att_seq& s, uint32_t 
     return r;
 }
 
-// Cache row of a key of sequence `seq`; keys outside [lo, hi) are not looked up and read row 0, whose values are not used.
-// A table entry that names no page raises a fault and reads row 0 as well.
-DEV uint32_t att_row(const apk_attend_args& a, const uint32_t* tab, int32_t key, int32_t lo, int32_t hi) {
-    if (key < lo || key >= hi) return 0;
+// The cache row of a key in two steps, so that the table entry is under way while the loads issued before it are (loads
+// return in order: an entry used at once would wait for all of them).  Keys outside [lo, hi) read row 0, whose values are
+// not used; a table entry that names no page reads row 0 as well, and is reported once at the end.
+struct att_entry {
+    uint32_t e, off;
+};
+DEV att_entry att_look(const apk_attend_args& a, const uint32_t* tab, int32_t key, int32_t lo, int32_t hi) {
     uint32_t idx, off;
-    split_key(a, (uint32_t)key, idx, off);
-    const uint32_t e = tab[idx];
-    if (e >= a.n_pages) {
-        atomicOr(a.fault, APK_FAULT_CACHE_RANGE);
-        return 0;
-    }
-    return e * a.page + off;
+    const bool in = key >= lo && key < hi;
+    split_key(a, in ? (uint32_t)key : 0u, idx, off);
+    return {tab[idx], in ? off : 0xffffffffu};
+}
+DEV uint32_t att_row(const apk_attend_args& a, att_entry t, bool& bad) {
+    const bool in = t.off != 0xffffffffu, ok = in && t.e < a.n_pages;
+    bad |= in && !ok;
+    return ok ? t.e * a.page + t.off : 0;
+}
+DEV void att_report(const apk_attend_args& a, bool bad) {
+    if (bad) atomicOr(a.fault, APK_FAULT_CACHE_RANGE);
 }
 
 // ------------------------------------------------------------------------------------------- query fragments
@@ -270,233 +352,7 @@ template <> __device__ __forceinline__ void att_store4<f16_t>(f16_t* p, const fl
 }
 template <> __device__ __forceinline__ void att_store4<float>(float* p, const float* v) { io<float>::store(p, v); }
 
-// ------------------------------------------------------------------------------------------- single tokens
-// One workgroup per (sequence, kv head, tile of up to 16 query heads, part of the keys); its waves take blocks of 32 keys
-// in turn and are joined through LDS at the end.  K and V go from memory straight to registers: a wave's K block is the
-// first operand of 16x16x32 products as it lies (16 bytes of a key a lane), its V block becomes one by an in-lane
-// transpose (8 keys x 8 channels a lane).  Bound by the stream of K and V.
-template <typename T, int HD, int W>
-DEV void attend_token_body(const apk_attend_args& a, float* smem) {
-    constexpr int KF = HD / 32;           // K fragments of 16 keys
-    constexpr int CH = HD / 16;           // channels a lane holds of a V row
-    constexpr int NQ = att_q<T>::N;
-    const uint32_t H = a.n_kv * a.head_tiles;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
-    att_item it;
-    if (!att_find<false>(a, blockIdx.x / H, it)) return;
-    const uint32_t hh = blockIdx.x % H, kvh = hh / a.head_tiles, ht = hh % a.head_tiles;
-    const uint32_t rows_here = min(APK_ATT_TOKEN_ROWS, a.group - ht * APK_ATT_TOKEN_ROWS);
-    const att_span sp = att_tile_span(a, it.s, it.part, 0, 0);
-    const uint32_t* tab = a.table + (uint64_t)it.seq * a.max_pages;
-    const uint64_t kv_stride = (uint64_t)a.n_kv * HD;
-    const f16_t* kb = (const f16_t*)a.k + (uint64_t)kvh * HD;
-    const f16_t* vb = (const f16_t*)a.v + (uint64_t)kvh * HD;
-    const uint64_t qat = (uint64_t)it.s.row0 * a.n_q * HD + (uint64_t)(kvh * a.group + ht * APK_ATT_TOKEN_ROWS) * HD;
-    const T* qb = (const T*)a.q + qat;
-
-    f16x8 qf[KF][NQ];
-    float qinv = 1.f;
-    {
-        const bool on = n16 < rows_here;
-        float mul = 1.f;
-        if constexpr (NQ == 2) {
-            float mx = 0.f;
-#pragma unroll
-            for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qb + n16 * HD + s * 32 + g * 8, on));
-            mx = max_xor<32>(max_xor<16>(mx));
-            att_q_scale(mx, mul, qinv);
-        }
-#pragma unroll
-        for (int s = 0; s < KF; s++) att_q<T>::load(qb + n16 * HD + s * 32 + g * 8, on, a.sign, mul, qf[s]);
-    }
-    const float c = a.c * qinv;
-
-    f32x4 o[CH];
-#pragma unroll
-    for (int i = 0; i < CH; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = NEG_INF, l = 0.f;
-
-    typedef uint32_t vrow_t __attribute__((ext_vector_type(CH / 2)));
-    const int32_t k_end = min((int32_t)(sp.u1 * APK_ATT_TOKEN_UNIT), sp.hi);
-    int32_t key0 = (int32_t)(sp.u0 * APK_ATT_TOKEN_UNIT) + (int32_t)wave * 32;
-    const int32_t k_lo = max(sp.lo, (int32_t)(sp.u0 * APK_ATT_TOKEN_UNIT));
-    f16x8 kf[2][KF];
-    vrow_t vr[8];
-    auto load_k = [&](uint32_t row) {
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-            const uint32_t r = __shfl(row, b * 16 + n16);
-            const f16_t* p = kb + (uint64_t)r * kv_stride + g * 8;
-#pragma unroll
-            for (int s = 0; s < KF; s++) kf[b][s] = *(const f16x8*)(p + s * 32);
-        }
-    };
-    auto load_v = [&](uint32_t row) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t r = __shfl(row, (j >> 2) * 16 + g * 4 + (j & 3));
-            const f16_t* p = vb + (uint64_t)r * kv_stride;
-            if constexpr (CH == 4) vr[j] = *(const vrow_t*)(p + n16 * 4);
-            if constexpr (CH == 8) vr[j] = *(const vrow_t*)(p + n16 * 8);
-            if constexpr (CH == 16) {
-                const u32x4 x = *(const u32x4*)(p + n16 * 8), y = *(const u32x4*)(p + 128 + n16 * 8);
-                vr[j] = vrow_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-            }
-        }
-    };
-    uint32_t row = 0;
-    if (key0 < k_end) {
-        row = att_row(a, tab, key0 + (int32_t)(lane & 31), k_lo, k_end);
-        load_k(row);
-        load_v(row);
-    }
-    while (key0 < k_end) {
-        const int32_t next = key0 + 32 * W;
-        const bool more = next < k_end;
-        uint32_t nrow = 0;
-        if (more) nrow = att_row(a, tab, next + (int32_t)(lane & 31), k_lo, k_end);
-        f32x4 s[2];
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-            s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < KF; i++)
-#pragma unroll
-                for (int t = 0; t < NQ; t++) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b][i], qf[i][t], s[b], 0, 0, 0);
-        }
-        if (more) load_k(nrow);
-        const bool edge = key0 < k_lo || key0 + 32 > k_end;
-        if (edge) {
-#pragma unroll
-            for (int b = 0; b < 2; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int32_t key = key0 + b * 16 + (int32_t)g * 4 + i;
-                    if (key < k_lo || key >= k_end) s[b][i] = NEG_INF;
-                }
-        }
-        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        mx = max_xor<32>(max_xor<16>(mx)) * c;
-        const float mn = fmaxf(m, mx);
-        const float ms = mn == NEG_INF ? 0.f : mn;
-        if (__any(mn > m)) {
-            const float alpha = exp2_hw(m - ms);
-            l *= alpha;
-#pragma unroll
-            for (int i = 0; i < CH; i++) o[i] *= alpha;
-            m = mn;
-        }
-        const float sub = kProbShift - ms;
-        f16x8 ph, pl;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float p = exp2_hw(__builtin_fmaf(s[j >> 2][j & 3], c, sub));
-            l += p;
-            ph[j] = (f16_t)p;
-            if constexpr (NQ == 2) pl[j] = (f16_t)(p - (float)ph[j]);
-        }
-        if (edge) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int32_t key = key0 + (j >> 2) * 16 + (int32_t)g * 4 + (j & 3);
-                if (key < k_lo || key >= k_end) vr[j] = (vrow_t)(0u);
-            }
-        }
-        f16x8 vt[CH];
-#pragma unroll
-        for (int w = 0; w < CH / 2; w++) {
-            u32x4 e, d;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                e[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w], vr[2 * j][w], 0x05040100u);
-                d[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w], vr[2 * j][w], 0x07060302u);
-            }
-            vt[2 * w] = __builtin_bit_cast(f16x8, e);
-            vt[2 * w + 1] = __builtin_bit_cast(f16x8, d);
-        }
-        if (more) load_v(nrow);
-#pragma unroll
-        for (int i = 0; i < CH; i++) {
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], ph, o[i], 0, 0, 0);
-            if constexpr (NQ == 2) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], pl, o[i], 0, 0, 0);
-        }
-        key0 = next;
-    }
-    l = sum_xor<32>(sum_xor<16>(l));
-
-    // join the waves: their maxima, then the sums of the rescaled outputs
-    const uint32_t R = rows_here;
-    float* sm_m = smem;               // [W][16]
-    float* sm_l = smem + W * 16;      // [W][16]
-    float* sm_o = smem + 2 * W * 16;  // [W][R][HD]
-    if (g == 0) sm_m[wave * 16 + n16] = m;
-    __syncthreads();
-    float M = NEG_INF;
-#pragma unroll
-    for (int w = 0; w < W; w++) M = fmaxf(M, sm_m[w * 16 + n16]);
-    const float f = m == NEG_INF ? 0.f : exp2_hw(m - M);
-    if (g == 0) sm_l[wave * 16 + n16] = l * f;
-    if (n16 < R) {
-        float* dst = sm_o + ((uint64_t)wave * R + n16) * HD;
-        // o[ci][i]: channel CHW * (4 g + i) + ci, the lanes of 256 channels holding two runs of eight 128 apart
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int ci = 0; ci < CH; ci++) {
-                const int m16 = (int)g * 4 + i;
-                const int chan = CH == 16 ? (ci >> 3) * 128 + m16 * 8 + (ci & 7) : m16 * CH + ci;
-                dst[chan] = o[ci][i] * f;
-            }
-    }
-    __syncthreads();
-    const bool split = it.s.parts > 1;
-    float* part = a.part + ((uint64_t)it.slot * H + hh) * ((uint64_t)APK_ATT_TOKEN_ROWS * (HD + 2));
-    for (uint32_t i = threadIdx.x; i < R * (HD / 4); i += W * 64) {
-        const uint32_t r = i / (HD / 4), col = (i % (HD / 4)) * 4;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        float ls = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            v += *(const f32x4*)(sm_o + ((uint64_t)w * R + r) * HD + col);
-            ls += sm_l[w * 16 + r];
-        }
-        if (split) {
-            *(f32x4*)(part + r * HD + col) = v;
-            if (col == 0) {
-                float mm = NEG_INF;
-#pragma unroll
-                for (int w = 0; w < W; w++) mm = fmaxf(mm, sm_m[w * 16 + r]);
-                part[APK_ATT_TOKEN_ROWS * HD + r] = mm;
-                part[APK_ATT_TOKEN_ROWS * (HD + 1) + r] = ls;
-            }
-        } else {
-            const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);
-            float t[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-            att_store4<T>((T*)a.out + qat + (uint64_t)r * HD + col, t);
-        }
-    }
-}
-extern __shared__ float att_smem[];
-#define ATTEND_TOKEN(T, t, HD, W)                                                                                            \
-    extern "C" __global__ __launch_bounds__(W * 64) void apk_attend_token_##t##_hd##HD##_w##W(apk_attend_args a) {           \
-        attend_token_body<T, HD, W>(a, att_smem);                                                                            \
-    }
-#define ATTEND_TOKEN_ALL(W) \
-    ATTEND_TOKEN(f16_t, f16, 64, W) ATTEND_TOKEN(f16_t, f16, 128, W) ATTEND_TOKEN(f16_t, f16, 256, W) \
-    ATTEND_TOKEN(float, f32, 64, W) ATTEND_TOKEN(float, f32, 128, W) ATTEND_TOKEN(float, f32, 256, W)
-ATTEND_TOKEN_ALL(4)
-
-// ------------------------------------------------------------------------------------------- chunks of new tokens
-// One workgroup of four waves per (sequence, kv head, tile of 128 flat (token, head) rows, part of the keys).  Units of
-// BN keys go through LDS (fetched into registers while the unit before is worked on, two buffers, one barrier a unit); a
-// wave holds 32 rows.  K rows are the first operand of 32x32x16 products as they lie; V comes out of LDS transposed
-// (ds_read_b64_tr_b16), in the key order in which a lane holds its probabilities.  The 16-byte chunks of LDS row r are
-// permuted by f(r), so that both kinds of reads meet all banks.  Bound by the matrix and vector pipes together: for 32
-// rows x 32 keys x 128 channels 512 cycles of products stand next to about as many for the softmax.
-template <int HD> DEV uint32_t att_swz(uint32_t r) {
-    if constexpr (HD == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
-    else return ((r & 3) << 2) | ((r >> 2) & 3);
-}
+// ------------------------------------------------------------------------------------------- few rows
 DEV bool att_nonfinite(u32x4 t) {  // any of eight fp16 values infinite or NaN
     bool b = false;
 #pragma unroll
@@ -511,6 +367,344 @@ DEV u32x4 att_clear_nonfinite(u32x4 t) {
     }
     return t;
 }
+// Single tokens, and chunks of a few: tiles of 16 NB flat rows.  A workgroup of W waves takes `heads` kv heads of one tile
+// and part, W / heads waves to a head, each of them blocks of 32 keys in turn; so a workgroup reads whole rows of the
+// cache where there are W heads or more, and its waves need not be joined.  K and V go from memory straight to registers:
+// a wave's K block is the first operand of 16x16x32 products as it lies (16 bytes of a key a lane), its V block becomes
+// one by an in-lane transpose (8 keys x 8 channels a lane).  K of the next block is under way from the moment K of this
+// one is used up, V likewise.  Bound by the stream of K and V.
+template <typename T, int HD, int NB, int W>
+DEV void attend_few_body(const apk_attend_args& a, float* smem) {
+    constexpr int KF = HD / 32;           // K fragments of 16 keys
+    constexpr int CH = HD / 16;           // channels a lane holds of a V row
+    constexpr int NQ = att_q<T>::N, R = 16 * NB;
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
+    const uint32_t hblocks = a.n_kv / a.heads, WK = W / a.heads;
+    const uint32_t kvh = blockIdx.x % hblocks * a.heads + wave % a.heads, wk = wave / a.heads, piece = blockIdx.x / hblocks;
+    uint64_t x0, x1, share;
+    const uint32_t all_tiles = att_share(a, piece, x0, x1, share);
+    const bool lists = threadIdx.x == 0 && blockIdx.x % hblocks == 0 && a.scratch;
+    if (lists && piece == 0) a.scratch[0] = a.list_tiles ? all_tiles : a.target;
+    if (lists && !a.list_tiles) a.scratch[16 + 8 * piece + 3] = 0;  // no tile that goes on in the next piece, so far
+    bool first_seg = true;
+    for (uint64_t x = x0; x < x1; first_seg = false) {
+    att_place it;
+    att_locate(a, x, it);
+    const uint64_t tile_end = it.begin + it.s.umax, seg_end = min(tile_end, x1);
+    const bool split = it.begin < x || tile_end > x1;
+    const uint32_t slot = 2 * piece + (first_seg ? 0 : 1);
+    if (lists && it.begin == x) {  // the tile begins here: its parts are this one and the first segments of the next pieces
+        uint32_t* d = a.scratch + 16 + 8 * (a.list_tiles ? it.number : piece);
+        const uint32_t parts = split ? 1 + (uint32_t)((tile_end - x1 + share - 1) / share) : 0;
+        if (a.list_tiles || split) {
+            *(u32x4*)d = u32x4{it.s.row0, it.s.m, it.tile, parts};
+            *(u32x4*)(d + 4) = u32x4{slot, 2 * (piece + 1), 2, 0};
+        }
+    }
+    const uint64_t flat_n = (uint64_t)it.s.m * a.group, flat0 = (uint64_t)it.tile * R;
+    const uint32_t rows_here = (uint32_t)min(flat_n - flat0, (uint64_t)R);
+    const uint32_t tok0 = (uint32_t)(flat0 / a.group), tok1 = (uint32_t)((flat0 + rows_here - 1) / a.group);
+    att_span sp = att_tile_span(a, it.s, 0, tok0, tok1);
+    sp.u1 = min(sp.u1, sp.u0 + (uint32_t)(seg_end - it.begin));
+    sp.u0 = min(sp.u1, sp.u0 + (uint32_t)(x - it.begin));
+    x = seg_end;
+    const uint32_t* tab = a.table + (uint64_t)it.seq * a.max_pages;
+    const uint64_t kv_stride = (uint64_t)a.n_kv * HD;
+    const f16_t* kb = (const f16_t*)a.k + (uint64_t)kvh * HD;
+    const f16_t* vb = (const f16_t*)a.v + (uint64_t)kvh * HD;
+
+    f16x8 qf[NB][KF][NQ];
+    float c[NB], m[NB], l[NB];
+    int32_t pos[NB];
+    uint64_t qat[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        const uint32_t flat = (uint32_t)flat0 + nb * 16 + n16, tok = flat / a.group;
+        const bool on = nb * 16 + n16 < rows_here;
+        qat[nb] = on ? ((uint64_t)(it.s.row0 + tok) * a.n_q + kvh * a.group + flat % a.group) * HD : 0;
+        pos[nb] = on ? it.s.p0 + (int32_t)tok : -1;
+        const T* qb = (const T*)a.q + qat[nb] + g * 8;
+        float mul = 1.f, inv = 1.f;
+        if constexpr (NQ == 2) {
+            float mx = 0.f;
+#pragma unroll
+            for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qb + s * 32, on));
+            att_q_scale(max_xor<32>(max_xor<16>(mx)), mul, inv);
+        }
+#pragma unroll
+        for (int s = 0; s < KF; s++) att_q<T>::load(qb + s * 32, on, a.sign, mul, qf[nb][s]);
+        c[nb] = a.c * inv;
+        m[nb] = NEG_INF;
+        l[nb] = 0.f;
+    }
+    f32x4 o[NB][CH];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int i = 0; i < CH; i++) o[nb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    typedef uint32_t vrow_t __attribute__((ext_vector_type(CH / 2)));
+    const int32_t k_end = min((int32_t)(sp.u1 * 32), sp.hi), k_lo = max(sp.lo, (int32_t)(sp.u0 * 32));
+    const int32_t key_first = (int32_t)(sp.u0 * 32 + wk * 32), stride = (int32_t)(32 * WK);
+    const int32_t tpos0 = it.s.p0 + (int32_t)tok0, tpos1 = it.s.p0 + (int32_t)tok1;
+    // some row of the tile does not see all keys of this block
+    auto is_partial = [&](int32_t key0) { return key0 + 31 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
+    f16x8 kf[2][KF];
+    vrow_t vr[8];
+    auto load_k = [&](uint32_t row) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const f16_t* p = kb + (uint64_t)__shfl(row, b * 16 + n16) * kv_stride + g * 8;
+#pragma unroll
+            for (int s = 0; s < KF; s++) kf[b][s] = *(const f16x8*)(p + s * 32);
+        }
+    };
+    auto load_v = [&](uint32_t row) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const f16_t* p = vb + (uint64_t)__shfl(row, (j >> 2) * 16 + g * 4 + (j & 3)) * kv_stride;
+            if constexpr (CH == 4) vr[j] = *(const vrow_t*)(p + n16 * 4);
+            if constexpr (CH == 8) vr[j] = *(const vrow_t*)(p + n16 * 8);
+            if constexpr (CH == 16) {
+                const u32x4 x = *(const u32x4*)(p + n16 * 8), y = *(const u32x4*)(p + 128 + n16 * 8);
+                vr[j] = vrow_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            }
+        }
+    };
+    auto look = [&](int32_t key) { return att_look(a, tab, key + (int32_t)(lane & 31), k_lo, k_end); };
+    bool bad = false, odd = false;  // a table entry that names no page; a value of V that is not finite was cleared
+    att_entry ahead = {0, 0};       // the table entries of the block after the one that is worked on
+    int32_t key0 = key_first;
+    if (key0 < k_end) {
+        const att_entry t = look(key0);
+        ahead = look(key0 + stride);
+        const uint32_t row = att_row(a, t, bad);
+        load_k(row);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(row);
+    }
+    while (key0 < k_end) {
+        const int32_t next = key0 + stride;
+        f32x4 s[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                s[nb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < KF; i++)
+#pragma unroll
+                    for (int t = 0; t < NQ; t++) s[nb][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b][i], qf[nb][i][t], s[nb][b], 0, 0, 0);
+            }
+        // (without a condition on there being a next block: behind the last one this reads row 0, and a condition here
+        // makes the compiler copy what it loads, that is wait for it)
+        const uint32_t nrow = att_row(a, ahead, bad);
+        ahead = look(next + stride);
+        load_k(nrow);
+        __builtin_amdgcn_sched_barrier(0);  // K before V, so that K can be waited for with V under way
+        const bool partial = key0 < k_lo || is_partial(key0);  // (a block that ends behind the last key is one)
+        if (partial) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int32_t key = key0 + b * 16 + (int32_t)g * 4 + i;
+                        if (key < k_lo || key > pos[nb] || (a.window && key <= pos[nb] - (int32_t)a.window)) s[nb][b][i] = NEG_INF;
+                    }
+        }
+        f16x8 ph[NB], pl[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            float mx = fmaxf(fmaxf(fmaxf(s[nb][0][0], s[nb][0][1]), fmaxf(s[nb][0][2], s[nb][0][3])), fmaxf(fmaxf(s[nb][1][0], s[nb][1][1]), fmaxf(s[nb][1][2], s[nb][1][3])));
+            mx = max_xor<32>(max_xor<16>(mx)) * c[nb];
+            const float mn = fmaxf(m[nb], mx), ms = mn == NEG_INF ? 0.f : mn;
+            if (__any(mn > m[nb])) {
+                const float alpha = exp2_hw(m[nb] - ms);
+                l[nb] *= alpha;
+#pragma unroll
+                for (int i = 0; i < CH; i++) o[nb][i] *= alpha;
+                m[nb] = mn;
+            }
+            const float sub = kProbShift - ms;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float p = exp2_hw(__builtin_fmaf(s[nb][j >> 2][j & 3], c[nb], sub));
+                l[nb] += p;
+                ph[nb][j] = (f16_t)p;
+                if constexpr (NQ == 2) pl[nb][j] = (f16_t)(p - (float)ph[nb][j]);
+            }
+        }
+        if (partial) {  // keys that no row sees: zero; values that are not finite: see below
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int32_t key = key0 + (j >> 2) * 16 + (int32_t)g * 4 + (j & 3);
+                if (key < k_lo || key >= k_end) vr[j] = (vrow_t)(0u);
+#pragma unroll
+                for (int w = 0; w < CH / 2; w++) {
+                    const uint32_t t = vr[j][w];
+                    const bool lo = (t & 0x7c00u) == 0x7c00u, hi = (t & 0x7c000000u) == 0x7c000000u;
+                    odd |= lo || hi;
+                    vr[j][w] = t & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
+                }
+            }
+        }
+        f16x8 vt[CH];
+#pragma unroll
+        for (int w = 0; w < CH / 2; w++) {
+            u32x4 e, d;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                e[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w], vr[2 * j][w], 0x05040100u);
+                d[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w], vr[2 * j][w], 0x07060302u);
+            }
+            vt[2 * w] = __builtin_bit_cast(f16x8, e);
+            vt[2 * w + 1] = __builtin_bit_cast(f16x8, d);
+        }
+        load_v(nrow);
+#pragma unroll
+        for (int i = 0; i < CH; i++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                o[nb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], ph[nb], o[nb][i], 0, 0, 0);
+                if constexpr (NQ == 2) o[nb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], pl[nb], o[nb][i], 0, 0, 0);
+            }
+        key0 = next;
+        __builtin_amdgcn_sched_barrier(0);  // V is issued here, not at the head of the next round
+    }
+    att_report(a, bad);
+    // o[nb][ci][i]: row nb * 16 + n16, channel chan(4 g + i, ci); heads of 256 channels hold two runs of eight, 128 apart
+    auto chan = [&](int i, int ci) { return CH == 16 ? (ci >> 3) * 128 + ((int)g * 4 + i) * 8 + (ci & 7) : ((int)g * 4 + i) * CH + ci; };
+    // A value of V that is not finite, in a block that some rows see only in part, was cleared on its way in, so that it
+    // met no weight of zero; the rows that do see it get it here, as it is (any weight above zero leaves it so).
+    if (__any(odd)) {
+#pragma unroll 1
+        for (int32_t k0 = key_first; k0 < k_end; k0 += stride) {
+            if (!(k0 < k_lo || is_partial(k0))) continue;
+#pragma unroll 1
+            for (int32_t key = max(k0, k_lo); key < min(k0 + 32, k_end); key++) {
+                bool no = false;
+                const f16_t* p = vb + (uint64_t)att_row(a, att_look(a, tab, key, k_lo, k_end), no) * kv_stride;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int ci = 0; ci < CH; ci++) {
+                        const float x = (float)p[chan(i, ci)];
+                        const bool nonfinite = !(__builtin_fabsf(x) < __builtin_inff());
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++)
+                            if (nonfinite && key <= pos[nb] && !(a.window && key <= pos[nb] - (int32_t)a.window)) o[nb][ci][i] += x;
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) l[nb] = sum_xor<32>(sum_xor<16>(l[nb]));
+    float* part = att_part(a, split ? slot : 0, kvh);
+    if (WK == 1) {  // a wave has the whole result of its head
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const uint32_t r = nb * 16 + n16;
+            if (r >= rows_here) continue;
+            const float f = split ? 1.f : att_inverse(l[nb]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int ci = 0; ci < CH; ci += 4) {
+                    float t[4] = {o[nb][ci][i] * f, o[nb][ci + 1][i] * f, o[nb][ci + 2][i] * f, o[nb][ci + 3][i] * f};
+                    if (split) io<float>::store(part + (uint64_t)r * HD + chan(i, ci), t);
+                    else att_store4<T>((T*)a.out + qat[nb] + chan(i, ci), t);
+                }
+            if (split && g == 0) {
+                part[R * HD + r] = m[nb];
+                part[R * (HD + 1) + r] = l[nb];
+            }
+        }
+        continue;
+    }
+    // join the waves of a head: their maxima, then the sums of the rescaled outputs
+    const uint32_t RR = rows_here;
+    float* sm_m = smem;              // [W][R]
+    float* sm_l = smem + W * R;      // [W][R]
+    float* sm_o = smem + 2 * W * R;  // [W][RR][HD]
+    const uint32_t hl = wave % a.heads;  // the head's waves: hl, hl + heads, ...
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+        if (g == 0) sm_m[wave * R + nb * 16 + n16] = m[nb];
+    __syncthreads();
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        const uint32_t r = nb * 16 + n16;
+        float M = NEG_INF;
+        for (uint32_t w = hl; w < W; w += a.heads) M = fmaxf(M, sm_m[w * R + r]);
+        const float f = m[nb] == NEG_INF ? 0.f : exp2_hw(m[nb] - M);
+        if (g == 0) sm_l[wave * R + r] = l[nb] * f;
+        if (r < RR) {
+            float* dst = sm_o + ((uint64_t)wave * RR + r) * HD;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int ci = 0; ci < CH; ci += 4)
+                    *(f32x4*)(dst + chan(i, ci)) = f32x4{o[nb][ci][i] * f, o[nb][ci + 1][i] * f, o[nb][ci + 2][i] * f, o[nb][ci + 3][i] * f};
+        }
+    }
+    __syncthreads();
+    const uint32_t kvh0 = blockIdx.x % hblocks * a.heads;
+    for (uint32_t i = threadIdx.x; i < a.heads * RR * (HD / 4); i += W * 64) {
+        const uint32_t col = i % (HD / 4) * 4, r = i / (HD / 4) % RR, h = i / (HD / 4) / RR;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        float ls = 0.f, mm = NEG_INF;
+        for (uint32_t w = h; w < W; w += a.heads) {
+            v += *(const f32x4*)(sm_o + ((uint64_t)w * RR + r) * HD + col);
+            ls += sm_l[w * R + r];
+            mm = fmaxf(mm, sm_m[w * R + r]);
+        }
+        if (split) {
+            float* to = att_part(a, slot, kvh0 + h);
+            *(f32x4*)(to + (uint64_t)r * HD + col) = v;
+            if (col == 0) {
+                to[R * HD + r] = mm;
+                to[R * (HD + 1) + r] = ls;
+            }
+        } else {
+            const float inv = att_inverse(ls);
+            const uint32_t flat = (uint32_t)flat0 + r;
+            float t[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+            att_store4<T>((T*)a.out + ((uint64_t)(it.s.row0 + flat / a.group) * a.n_q + (kvh0 + h) * a.group + flat % a.group) * HD + col, t);
+        }
+    }
+    __syncthreads();  // the next segment writes there again
+    }
+}
+extern __shared__ float att_smem[];
+#define ATTEND_FEW(HD, NB, W)                                                                                                \
+    extern "C" __global__ __launch_bounds__(W * 64, W / 4) void apk_attend_few_f16_hd##HD##_b##NB(apk_attend_args a) {       \
+        attend_few_body<f16_t, HD, NB, W>(a, att_smem);                                                                      \
+    }                                                                                                                        \
+    extern "C" __global__ __launch_bounds__(W * 64, W / 4) void apk_attend_few_f32_hd##HD##_b##NB(apk_attend_args a) {       \
+        attend_few_body<float, HD, NB, W>(a, att_smem);                                                                      \
+    }
+ATTEND_FEW(64, 1, 8)
+ATTEND_FEW(64, 2, 8)
+ATTEND_FEW(64, 4, 8)
+ATTEND_FEW(128, 1, 8)
+ATTEND_FEW(128, 2, 8)
+ATTEND_FEW(128, 4, 4)
+ATTEND_FEW(256, 1, 4)
+ATTEND_FEW(256, 2, 4)
+
+// ------------------------------------------------------------------------------------------- chunks of new tokens
+// One workgroup of four waves per (sequence, kv head, tile of 128 flat (token, head) rows, part of the keys).  Units of
+// BN keys go through LDS (fetched into registers while the unit before is worked on, two buffers, one barrier a unit); a
+// wave holds 32 rows.  K rows are the first operand of 32x32x16 products as they lie; V comes out of LDS transposed
+// (ds_read_b64_tr_b16), in the key order in which a lane holds its probabilities.  The 16-byte chunks of LDS row r are
+// permuted by f(r), so that both kinds of reads meet all banks.  Bound by the matrix and vector pipes together: for 32
+// rows x 32 keys x 128 channels 512 cycles of products stand next to about as many for the softmax.
+template <int HD> DEV uint32_t att_swz(uint32_t r) {
+    if constexpr (HD == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+}
 template <typename T, int HD, int BN>
 DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
     constexpr int KF = HD / 16, NQ = att_q<T>::N, KB = BN / 32, HB = HD / 32, CPR = HD / 8;
@@ -519,7 +713,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
     f16_t* const sk = smem;                    // [2][BN][HD]
     f16_t* const sv = smem + 2 * BN * HD;      // [2][BN][HD]
     att_item it;
-    if (!att_find<false>(a, blockIdx.x / H, it)) return;
+    if (!att_find(a, blockIdx.x / H, it)) return;
     const uint32_t kvh = blockIdx.x % H;
     const uint64_t flat_n = (uint64_t)it.s.m * a.group, flat0 = (uint64_t)it.tile * APK_ATT_CHUNK_ROWS;
     const uint32_t tok0 = (uint32_t)(flat0 / a.group);
@@ -568,20 +762,18 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
     auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
     bool odd = false;  // a value of V that is not finite was cleared
     // staging: thread t takes chunks t, t + 256, ... of a unit
-    uint32_t rows[NCH];
+    att_entry ent[NCH];
+    bool bad = false;
     u32x4 rk[NCH], rv[NCH];
     auto look = [&](uint32_t u) {
 #pragma unroll
-        for (int i = 0; i < NCH; i++) {
-            const uint32_t r = (i * 256 + tid) / CPR;
-            rows[i] = att_row(a, tab, (int32_t)(u * BN + r), sp.lo, sp.hi);
-        }
+        for (int i = 0; i < NCH; i++) ent[i] = att_look(a, tab, (int32_t)(u * BN + (i * 256 + tid) / CPR), sp.lo, sp.hi);
     };
     auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < NCH; i++) {
             const uint32_t p = i * 256 + tid, r = p / CPR, ch = (p % CPR) ^ att_swz<HD>(r);
-            const uint64_t at = (uint64_t)rows[i] * kv_stride + ch * 8;
+            const uint64_t at = (uint64_t)att_row(a, ent[i], bad) * kv_stride + ch * 8;
             rk[i] = *(const u32x4*)(kb + at);
             rv[i] = *(const u32x4*)(vb + at);
         }
@@ -699,6 +891,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
         if (u + 1 < sp.u1) stage(u + 1);
         __syncthreads();
     }
+    att_report(a, bad);
     // A value of V that is not finite, in a unit that some rows see only in part, was cleared on its way in, so that it
     // met no weight of zero; the rows that do see it get it here, as it is (any weight above zero leaves it so).
     if (__syncthreads_or(odd)) {
@@ -708,7 +901,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
 #pragma unroll 1
             for (int32_t key = (int32_t)(u * BN); key < (int32_t)(u * BN) + BN; key++) {
                 if (key < sp.lo || key > pos || (a.window && key <= pos_lo)) continue;
-                const f16_t* p = vb + (uint64_t)att_row(a, tab, key, sp.lo, sp.hi) * kv_stride + 4 * hf;
+                const f16_t* p = vb + (uint64_t)att_row(a, att_look(a, tab, key, sp.lo, sp.hi), bad) * kv_stride + 4 * hf;
 #pragma unroll
                 for (int hb = 0; hb < HB; hb++)
 #pragma unroll
@@ -725,7 +918,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
     if (!on) return;
     if (it.s.parts > 1) {
         const uint32_t r = wave * 32 + n32;
-        float* part = a.part + ((uint64_t)it.slot * H + kvh) * ((uint64_t)APK_ATT_CHUNK_ROWS * (HD + 2));
+        float* part = att_part(a, it.slot, kvh);
 #pragma unroll
         for (int hb = 0; hb < HB; hb++)
 #pragma unroll
@@ -737,7 +930,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
         }
         return;
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const float inv = att_inverse(l);
     T* out = (T*)a.out + qat;
 #pragma unroll
     for (int hb = 0; hb < HB; hb++)
@@ -756,69 +949,124 @@ ATTEND_CHUNK(float, f32, 128, 64, 1)
 ATTEND_CHUNK(float, f32, 256, 32, 1)
 
 // ------------------------------------------------------------------------------------------- joining the parts
-// The tiles that were cut, and only those: a wave (WPR = 1) or a workgroup of four (WPR = 4: single tokens, few rows of
-// many parts) per row.  Bound by its launch.
-template <typename T, int WPR>
+// The tiles that were cut: a workgroup of eight waves takes join_rows (8 or 1) rows of one listed tile and kv head.  Of up
+// to 32 parts a wave joins a row on its own, hd / 4 lanes to a part; of more the whole workgroup shares the parts of one
+// row after the other, so that the loads of all of them are under way together.
+template <typename T>
 DEV void attend_join_body(const apk_attend_args& a) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t per_tile = WPR == 4 ? a.tile_rows : a.tile_rows / 4;  // workgroups of a tile
-    const uint32_t H = a.n_kv * a.head_tiles, t = blockIdx.x / per_tile;
-    att_item it;
-    if (!att_find<true>(a, t / H, it)) return;
-    const uint32_t hh = t % H, kvh = hh / a.head_tiles, ht = hh % a.head_tiles, hd = a.hd;
-    const uint32_t r = WPR == 4 ? blockIdx.x % per_tile : (blockIdx.x % per_tile) * 4 + wave;
-    uint64_t qat;
-    if (a.q_off) {
-        const uint64_t flat = (uint64_t)it.tile * a.tile_rows + r;
-        if (flat >= (uint64_t)it.s.m * a.group) return;
-        qat = ((uint64_t)(it.s.row0 + (uint32_t)(flat / a.group)) * a.n_q + kvh * a.group + (uint32_t)(flat % a.group)) * hd;
-    } else {
-        if (ht * APK_ATT_TOKEN_ROWS + r >= a.group) return;
-        qat = ((uint64_t)it.s.row0 * a.n_q + kvh * a.group + ht * APK_ATT_TOKEN_ROWS + r) * hd;
-    }
-    const uint32_t parts = it.s.parts;
-    const uint64_t slot_floats = (uint64_t)a.tile_rows * (hd + 2);
-    const float* base = a.part + ((uint64_t)it.slot * H + hh) * slot_floats;
-    const uint64_t step = (uint64_t)H * slot_floats;
-    const float* mp = base + (uint64_t)a.tile_rows * hd + r;
-    float M = NEG_INF;
-    for (uint32_t p = lane; p < parts; p += 64) M = fmaxf(M, mp[p * step]);
-    M = wave_max_f32(M);
-    const float Ms = M == NEG_INF ? 0.f : M;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    const uint32_t col = lane * 4;
-    const bool on = col < hd;
-#pragma unroll 4
-    for (uint32_t p = WPR == 1 ? 0 : wave; p < parts; p += WPR) {
-        const float w = exp2_hw(mp[p * step] - Ms);
-        l = __builtin_fmaf(mp[p * step + a.tile_rows], w, l);
-        const f32x4 v = *(const f32x4*)(base + p * step + (uint64_t)r * hd + (on ? col : 0));
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6), hd = a.hd, R = a.tile_rows;
+    const uint32_t per_tile = R / a.join_rows, x = blockIdx.x / per_tile;
+    const uint32_t kvh = x % a.n_kv, j = x / a.n_kv, r0 = blockIdx.x % per_tile * a.join_rows;
+    if (j >= a.scratch[0]) return;
+    const uint32_t* d = a.scratch + 16 + 8 * j;
+    const uint32_t row0 = d[0], m = d[1], tile = d[2], parts = d[3], slot0 = d[4], slot1 = d[5], step = d[6];
+    const uint64_t flat0 = (uint64_t)tile * R + r0, flat_n = (uint64_t)m * a.group;
+    if (parts < 2 || flat0 >= flat_n) return;
+    const uint32_t rows = (uint32_t)min((uint64_t)a.join_rows, flat_n - flat0);
+    const uint64_t to = (uint64_t)a.n_kv * R * (hd + 2);  // floats from slot to slot
+    const float* base = att_part(a, 0, kvh);
+    auto slot_of = [&](uint32_t p) { return base + (uint64_t)(p ? slot1 + (p - 1) * step : slot0) * to; };
+    auto finish = [&](uint32_t r, uint32_t col, f32x4 t, float l) {
+        const uint64_t flat = flat0 + r;
+        const float inv = att_inverse(l);
+        float v[4] = {t.x * inv, t.y * inv, t.z * inv, t.w * inv};
+        att_store4<T>((T*)a.out + ((uint64_t)(row0 + (uint32_t)(flat / a.group)) * a.n_q + kvh * a.group + (uint32_t)(flat % a.group)) * hd + col, v);
+    };
+    auto add = [](f32x4& acc, f32x4 v, float w) {
         acc.x = __builtin_fmaf(v.x, w, acc.x);
         acc.y = __builtin_fmaf(v.y, w, acc.y);
         acc.z = __builtin_fmaf(v.z, w, acc.z);
         acc.w = __builtin_fmaf(v.w, w, acc.w);
+    };
+    const uint32_t per = hd / 4, col = tid % per * 4;  // lanes of a part (16, 32 or 64)
+    if (parts <= 32 && a.join_rows > 1) {
+        const uint32_t r = wave;
+        if (r >= rows) return;
+        const uint32_t groups = 64 / per, grp = lane / per;
+        float mp = NEG_INF, lp = 0.f;  // of part `lane`
+        if (lane < parts) {
+            const float* q = slot_of(lane) + (uint64_t)R * hd + r0 + r;
+            mp = q[0];
+            lp = q[R];
+        }
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        float M = NEG_INF, w = 0.f;
+        for (uint32_t p0 = 0; p0 < parts; p0 += 4 * groups) {
+            f32x4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = *(const f32x4*)(slot_of(min(p0 + k * groups + grp, parts - 1)) + (uint64_t)(r0 + r) * hd + col);
+            if (p0 == 0) {
+                M = wave_max_f32(mp);
+                w = exp2_hw(mp - (M == NEG_INF ? 0.f : M));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t p = p0 + k * groups + grp;
+                const float wp = __shfl(w, p & 63);
+                if (p < parts) add(acc, v[k], wp);
+            }
+        }
+        const float l = group_sum<64>(lane < parts ? lp * w : 0.f);
+        for (uint32_t g = per; g < 64; g <<= 1) {
+            acc.x += __shfl_xor(acc.x, g);
+            acc.y += __shfl_xor(acc.y, g);
+            acc.z += __shfl_xor(acc.z, g);
+            acc.w += __shfl_xor(acc.w, g);
+        }
+        if (grp == 0) finish(r, col, acc, l);
+        return;
     }
-    if constexpr (WPR == 4) {
-        __shared__ f32x4 so[4][64];
-        __shared__ float sl[4];
-        so[wave][lane] = acc;
-        if (lane == 0) sl[wave] = l;
+    const uint32_t groups = 512 / per, grp = tid / per;
+    __shared__ float sw[512], sred[8];
+    __shared__ f32x4 so[512];
+    for (uint32_t r = 0; r < rows; r++) {
+        float M = NEG_INF;
+        for (uint32_t p = tid; p < parts; p += 512) M = fmaxf(M, slot_of(p)[(uint64_t)R * hd + r0 + r]);
+        M = wave_max_f32(M);
+        if (lane == 0) sred[wave] = M;
         __syncthreads();
-        if (wave) return;
-        acc = (so[0][lane] + so[1][lane]) + (so[2][lane] + so[3][lane]);
-        l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    }
-    if (on) {
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-        att_store4<T>((T*)a.out + qat + col, v);
+#pragma unroll
+        for (int w = 0; w < 8; w++) M = fmaxf(M, sred[w]);
+        const float Ms = M == NEG_INF ? 0.f : M;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+        for (uint32_t p0 = 0; p0 < parts; p0 += 512) {
+            const uint32_t n = min(512u, parts - p0);
+            __syncthreads();
+            if (tid < n) {
+                const float* q = slot_of(p0 + tid) + (uint64_t)R * hd + r0 + r;
+                const float w = exp2_hw(q[0] - Ms);
+                sw[tid] = w;
+                l = __builtin_fmaf(q[R], w, l);
+            }
+            __syncthreads();
+            for (uint32_t p = grp; p < n; p += 8 * groups) {
+                f32x4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = *(const f32x4*)(slot_of(p0 + min(p + k * groups, n - 1)) + (uint64_t)(r0 + r) * hd + col);
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (p + k * groups < n) add(acc, v[k], sw[p + k * groups]);
+            }
+        }
+        l = group_sum<64>(l);
+        so[tid] = acc;
+        __syncthreads();
+        if (lane == 0) sred[wave] = l;
+        __syncthreads();
+        if (tid < per) {
+            float ls = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; w++) ls += sred[w];
+            f32x4 t = so[tid];
+            for (uint32_t g = 1; g < groups; g++) t += so[g * per + tid];
+            finish(r, col, t, ls);
+        }
+        __syncthreads();
     }
 }
-extern "C" __global__ __launch_bounds__(256) void apk_attend_join_f16_w1(apk_attend_args a) { attend_join_body<f16_t, 1>(a); }
-extern "C" __global__ __launch_bounds__(256) void apk_attend_join_f32_w1(apk_attend_args a) { attend_join_body<float, 1>(a); }
-extern "C" __global__ __launch_bounds__(256) void apk_attend_join_f16_w4(apk_attend_args a) { attend_join_body<f16_t, 4>(a); }
-extern "C" __global__ __launch_bounds__(256) void apk_attend_join_f32_w4(apk_attend_args a) { attend_join_body<float, 4>(a); }
+extern "C" __global__ __launch_bounds__(512) void apk_attend_join_f16(apk_attend_args a) { attend_join_body<f16_t>(a); }
+extern "C" __global__ __launch_bounds__(512) void apk_attend_join_f32(apk_attend_args a) { attend_join_body<float>(a); }
 
 // ------------------------------------------------------------------------------------------- any head size
 // A workgroup of four waves per (row, query head), element by element: heads of other sizes than 64, 128 and 256 (up to
@@ -827,13 +1075,11 @@ template <typename T>
 DEV void attend_generic_body(const apk_attend_args& a, float* smem) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = a.hd;
     const uint32_t row = blockIdx.x / a.n_q, h = blockIdx.x % a.n_q, kvh = h / a.group;
-    att_seq s = {0, 0, 0, 0, 0, 1, 0};
+    att_seq s = {0, 0, 0, 0, 0, 0, 1};
     uint32_t seq = 0;
     bool found = false;
     for (uint32_t base = 0; base < a.n_seq && !found; base += 64) {
-        const uint32_t i = base + lane;
-        att_seq t = {0, 0, 0, 0, 0, 1, 0};
-        if (i < a.n_seq) t = att_load_seq(a, i);
+        const att_seq t = att_load_seq(a, base + lane);
         const uint64_t hit = __ballot(row >= t.row0 && row - t.row0 < t.m);
         if (hit) {
             const int l = __builtin_ctzll(hit);
@@ -860,9 +1106,10 @@ DEV void attend_generic_body(const apk_attend_args& a, float* smem) {
 #pragma unroll
     for (int i = 0; i < 16; i++) o[i] = 0.f;
     float m = NEG_INF, l = 0.f;
+    bool bad = false;
     for (int32_t k0 = lo + (int32_t)wave * 64; k0 < hi; k0 += 256) {
         const int32_t key = k0 + (int32_t)lane;
-        const uint32_t r = att_row(a, tab, key, lo, hi);
+        const uint32_t r = att_row(a, att_look(a, tab, key, lo, hi), bad);
         float x = NEG_INF;
         if (key < hi) {
             float d = 0.f;
@@ -885,6 +1132,7 @@ DEV void attend_generic_body(const apk_attend_args& a, float* smem) {
                 if (i * 64 + lane < hd) o[i] = __builtin_fmaf((float)vr[i * 64 + lane], pj, o[i]);
         }
     }
+    att_report(a, bad);
     l = group_sum<64>(l);
 #pragma unroll
     for (int i = 0; i < 16; i++)
@@ -901,7 +1149,7 @@ DEV void attend_generic_body(const apk_attend_args& a, float* smem) {
         f[w] = exp2_hw(sml[w * 2] - Ms);
         ls += sml[w * 2 + 1] * f[w];
     }
-    const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);
+    const float inv = att_inverse(ls);
     for (uint32_t i = threadIdx.x; i < hd; i += 256) {
         const float v = (so[i] * f[0] + so[hd + i] * f[1]) + (so[2 * hd + i] * f[2] + so[3 * hd + i] * f[3]);
         ((T*)a.out)[qat + i] = (T)(v * inv);
