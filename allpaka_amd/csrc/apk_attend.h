@@ -28,9 +28,11 @@ struct apk_attend_args {
     uint32_t heads;           // kv heads that a workgroup takes (few rows: a power of two that divides n_kv; chunks: 1)
     uint32_t target;          // chunks: tiles are cut until about this many workgroups have work; few rows: workgroups per block of heads
     uint32_t unit_min;        // fewest units worth a part of their own
+    uint32_t whole_units;     // few rows: not 0: every tile counts as this many units, and a piece is one tile
     uint32_t list_tiles;      // few rows: 1: the list has a place for every tile; 0: one for every workgroup
     uint32_t join_rows;       // rows that a workgroup of the joining launch takes
-    uint32_t tile_rows, unit; // rows and keys of the kernel's tile
+    uint32_t tile_rows, unit; // rows of a tile and keys of a unit, powers of two, and their logarithms
+    uint32_t tile_shift, unit_shift;
     float c;                  // |scale| * log2(e), kept above zero
     float sign;               // the sign of scale, applied to q
 };

@@ -1645,8 +1645,8 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
     std::string kernel;
     const double flat = (double)rows * a.group / (double)n_seq;  // rows of a kv head per sequence
     #ifndef V_NB1
-#define V_NB1 8.
-#define V_NB2 16.
+#define V_NB1 16.
+#define V_NB2 32.
 #endif
     const unsigned nb = !q_off || flat <= V_NB1 ? 1 : flat <= V_NB2 ? 2 : flat <= 64. && head_dim < 256 ? 4 : 0;
     if (nb) {
@@ -1670,12 +1670,29 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
         shmem = (unsigned)(4 * a.unit * head_dim * 2);
         kernel = "apk_attend_chunk_" + t_name + "_hd" + std::to_string(head_dim);
     }
-    const uint64_t tiles = rows * (uint64_t)a.group / a.tile_rows + n_seq, hblocks = n_kv / a.heads;
+    while ((1u << a.tile_shift) < a.tile_rows) a.tile_shift++;
+    while ((1u << a.unit_shift) < a.unit) a.unit_shift++;
+    const uint64_t tiles = rows * (uint64_t)a.group / a.tile_rows + n_seq;
     const uint64_t units = (max_pages * page_size + a.unit - 1) / a.unit;  // of a tile at most
     const size_t fit = (kAttendScratch - APK_ATT_PART_AT) / (2 * (size_t)a.tile_rows * (head_dim + 2) * 4);  // pairs of slots
     uint64_t items, listed;
     bool cut;
-    if (nb) {
+    // Caches that are short whatever their lengths, in launches that do not fill the chip: a workgroup per tile and head,
+    // its waves sharing the keys.  (600 keys, 8 kv heads: one launch, no joining launch.)
+    const bool whole = nb && units <= 32 && tiles * n_kv <= 256;
+    if (whole) {
+        const unsigned waves = block / 64;
+        a.heads = 1;
+        a.unit_min = a.whole_units = (uint32_t)units;
+        shmem = (unsigned)((2 * waves * a.tile_rows + waves * a.tile_rows * head_dim) * 4);
+    }
+    const uint64_t hblocks = n_kv / a.heads;
+    if (whole) {
+        a.target = (uint32_t)tiles;
+        items = tiles;
+        listed = 0;
+        cut = false;
+    } else if (nb) {
         // as many workgroups as fill the chip, each with at most two cut segments
         uint64_t t = (V_TT + hblocks - 1) / hblocks;
         if (t * n_kv > fit) t = fit / n_kv;
@@ -1697,7 +1714,7 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
         if (tiles * parts < items) items = tiles * parts;
         listed = (a.target + hblocks - 1) / hblocks;
         if (tiles < listed) listed = tiles;
-        a.join_rows = 8;
+        a.join_rows = 32;
         cut = parts > 1;
     }
     if (items * hblocks > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);

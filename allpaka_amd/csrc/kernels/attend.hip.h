@@ -95,14 +95,15 @@ DEV att_seq att_load_seq(const apk_attend_args& a, uint32_t i) {
     s.m = r1 - r0;
     s.n = (int32_t)n;
     s.p0 = (int32_t)n - (int32_t)s.m;
-    s.tiles = (uint32_t)(((uint64_t)s.m * a.group + a.tile_rows - 1) / a.tile_rows);
+    s.tiles = (s.m * a.group + a.tile_rows - 1) >> a.tile_shift;  // the host holds rows * group below 2^31
     uint32_t span = n;
     if (a.window) {  // keys that the rows of one tile see between them
         const uint64_t w = (uint64_t)a.window + a.tile_rows / a.group + 1 + a.unit;
         if (w < span) span = (uint32_t)w;
     }
-    s.umax = (span + a.unit - 1) / a.unit;
+    s.umax = (span + a.unit - 1) >> a.unit_shift;
     if (s.umax == 0) s.umax = 1;  // rows without keys are work too: they get zeros
+    if (a.whole_units) s.umax = a.whole_units;
     return s;
 }
 DEV uint32_t rl(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
@@ -193,80 +194,77 @@ DEV uint64_t wave_scan_u64(uint64_t v) {
     v = dpp_add64<0x143, 0xc>(v);
     return v;
 }
-// The piece [x0, x1) of the line of all units that workgroup w of `target` takes; empty for workgroups that are not needed.
-// Returns the number of tiles.
-DEV uint32_t att_share(const apk_attend_args& a, uint32_t w, uint64_t& x0, uint64_t& x1, uint64_t& share) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint64_t all = 0;
-    uint32_t tiles = 0;
-    for (uint32_t base = 0; base < a.n_seq; base += 64) {
-        const att_seq s = att_load_seq(a, base + lane);
-        all += rl64(wave_scan_u64((uint64_t)s.tiles * s.umax), 63);
-        tiles += rl(wave_scan_u32(s.tiles), 63);
+// The line of all units as a wave keeps it: 64 sequences at a time, one a lane, with the sums up to and with each.
+struct att_line {
+    uint32_t base;      // the sequence of lane 0
+    att_seq s;          // this lane's
+    uint64_t end;       // where its units end
+    uint32_t tiles;     // tiles up to and with it
+};
+DEV void att_line_load(const apk_attend_args& a, uint32_t base, uint64_t units, uint32_t tiles, att_line& ln) {
+    ln.base = base;
+    ln.s = att_load_seq(a, base + (threadIdx.x & 63));
+    ln.end = units + wave_scan_u64((uint64_t)ln.s.tiles * ln.s.umax);
+    ln.tiles = tiles + wave_scan_u32(ln.s.tiles);
+}
+// The piece [x0, x1) of the line that workgroup w of `target` takes; empty for workgroups that are not needed.  The line
+// is left at its beginning.  Returns the number of tiles.
+DEV uint32_t att_share(const apk_attend_args& a, uint32_t w, uint64_t& x0, uint64_t& x1, uint64_t& share, att_line& ln) {
+    att_line_load(a, 0, 0, 0, ln);
+    uint64_t all = rl64(ln.end, 63);
+    uint32_t tiles = rl(ln.tiles, 63);
+    for (uint32_t base = 64; base < a.n_seq; base += 64) {
+        att_line t;
+        att_line_load(a, base, all, tiles, t);
+        all = rl64(t.end, 63);
+        tiles = rl(t.tiles, 63);
     }
-    share = (all + a.target - 1) / a.target;
+    // (32-bit division where the numbers allow it)
+    share = all < 0x80000000u ? ((uint32_t)all + a.target - 1) / a.target : (all + a.target - 1) / a.target;
     if (share < a.unit_min) share = a.unit_min;
     x0 = min(all, share * w);
     x1 = min(all, x0 + share);
     return tiles;
 }
-// The tile that unit x of the line falls into, where its units begin, and its number among all tiles.
+// The tile that unit x of the line falls into (x does not go back), where its units begin, and its number among all tiles.
 struct att_place {
     uint32_t seq, tile, number;
     uint64_t begin;
     att_seq s;
 };
-DEV void att_locate(const apk_attend_args& a, uint64_t x, att_place& pl) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint64_t before = 0;
-    uint32_t tiles = 0;
-    for (uint32_t base = 0; base < a.n_seq; base += 64) {
-        const att_seq s = att_load_seq(a, base + lane);
-        const uint64_t cnt = (uint64_t)s.tiles * s.umax, inc = before + wave_scan_u64(cnt);
-        const uint32_t tinc = tiles + wave_scan_u32(s.tiles);
-        const uint64_t hit = __ballot(inc > x && inc - cnt <= x);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            pl.seq = base + (uint32_t)l;
-            pl.s.row0 = rl(s.row0, l);
-            pl.s.m = rl(s.m, l);
-            pl.s.n = (int32_t)rl((uint32_t)s.n, l);
-            pl.s.p0 = (int32_t)rl((uint32_t)s.p0, l);
-            pl.s.tiles = rl(s.tiles, l);
-            pl.s.umax = rl(s.umax, l);
-            pl.s.parts = 1;
-            const uint64_t first = rl64(inc - cnt, l);
-            pl.tile = (uint32_t)((x - first) / pl.s.umax);
-            pl.number = rl(tinc - s.tiles, l) + pl.tile;
-            pl.begin = first + (uint64_t)pl.tile * pl.s.umax;
-            return;
-        }
-        before = rl64(inc, 63);
-        tiles = rl(tinc, 63);
-    }
+DEV void att_locate(const apk_attend_args& a, uint64_t x, att_line& ln, att_place& pl) {
+    while (rl64(ln.end, 63) <= x && ln.base + 64 < a.n_seq) att_line_load(a, ln.base + 64, rl64(ln.end, 63), rl(ln.tiles, 63), ln);
+    const uint64_t cnt = (uint64_t)ln.s.tiles * ln.s.umax;
+    const int l = __builtin_ctzll(__ballot(ln.end > x && ln.end - cnt <= x) | (1ull << 63));
+    pl.seq = ln.base + (uint32_t)l;
+    pl.s.row0 = rl(ln.s.row0, l);
+    pl.s.m = rl(ln.s.m, l);
+    pl.s.n = (int32_t)rl((uint32_t)ln.s.n, l);
+    pl.s.p0 = (int32_t)rl((uint32_t)ln.s.p0, l);
+    pl.s.tiles = rl(ln.s.tiles, l);
+    pl.s.umax = rl(ln.s.umax, l);
+    pl.s.parts = 1;
+    const uint64_t first = rl64(ln.end - cnt, l), off = x - first;
+    pl.tile = off < 0x80000000u ? (uint32_t)off / pl.s.umax : (uint32_t)(off / pl.s.umax);
+    pl.number = rl(ln.tiles - ln.s.tiles, l) + pl.tile;
+    pl.begin = first + (uint64_t)pl.tile * pl.s.umax;
 }
 DEV float* att_part(const apk_attend_args& a, uint32_t slot, uint32_t kvh) {
     return (float*)((char*)a.scratch + APK_ATT_PART_AT) + ((uint64_t)slot * a.n_kv + kvh) * ((uint64_t)a.tile_rows * (a.hd + 2));
 }
 DEV float att_inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }  // no key: zeros; NaN stays
 
-// The keys [lo, hi) that any row of a tile sees (tok0 .. tok1: its first and last row of the sequence) and, of their
-// units, those of one part.
+// The keys [lo, hi) that any row of a tile sees (tok0 .. tok1: its first and last row of the sequence) and their units.
 struct att_span {
     int32_t lo, hi;    // keys
-    uint32_t u0, u1;   // units of this part: keys [u0 * unit, u1 * unit)
+    uint32_t u0, u1;   // units: keys [u0 * UNIT, u1 * UNIT)
 };
-DEV att_span att_tile_span(const apk_attend_args& a, const att_seq& s, uint32_t part, uint32_t tok0, uint32_t tok1) {
+template <int UNIT> DEV att_span att_tile_span(const apk_attend_args& a, const att_seq& s, uint32_t tok0, uint32_t tok1) {
     att_span r;
-    int64_t lo = a.window ? (int64_t)s.p0 + tok0 - (int64_t)a.window + 1 : 0;
-    int64_t hi = (int64_t)s.p0 + tok1 + 1;
-    r.lo = (int32_t)(lo < 0 ? 0 : lo);
-    r.hi = (int32_t)(hi < 0 ? 0 : hi);
-    uint32_t first = (uint32_t)r.lo / a.unit, last = ((uint32_t)r.hi + a.unit - 1) / a.unit;
-    if (last < first) last = first;
-    const uint64_t nu = last - first;
-    r.u0 = first + (uint32_t)(nu * part / s.parts);
-    r.u1 = first + (uint32_t)(nu * (part + 1) / s.parts);
+    r.lo = a.window ? max(0, s.p0 + (int32_t)tok0 - (int32_t)a.window + 1) : 0;
+    r.hi = max(0, s.p0 + (int32_t)tok1 + 1);
+    r.u0 = (uint32_t)r.lo / UNIT;
+    r.u1 = max(r.u0, ((uint32_t)r.hi + UNIT - 1) / UNIT);
     return r;
 }
 
@@ -292,41 +290,38 @@ DEV void att_report(const apk_attend_args& a, bool bad) {
 }
 
 // ------------------------------------------------------------------------------------------- query fragments
-// Eight consecutive elements of a query row as fp16: one fragment for fp16 rows, a high and a low one for f32 rows whose
-// elements are multiplied by `mul` (a power of two) first.
+// Eight consecutive elements of a query row, as they are loaded (zeros for a row that is not there) and as fp16: one
+// fragment for fp16 rows, a high and a low one for f32 rows, whose elements are multiplied by `mul` (a power of two) first.
 template <typename T> struct att_q;
 template <> struct att_q<f16_t> {
     static constexpr int N = 1;
-    DEV void load(const f16_t* p, bool on, float sign, float, f16x8* f) {
-        f16x8 t = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (on) t = *(const f16x8*)p;
-        f[0] = sign < 0.f ? -t : t;
-    }
-    DEV float absmax(const f16_t*, bool) { return 0.f; }
+    typedef f16x8 raw_t;
+    DEV raw_t load(const f16_t* p, bool on) { return on ? *(const f16x8*)p : f16x8{0, 0, 0, 0, 0, 0, 0, 0}; }
+    DEV float absmax(raw_t) { return 0.f; }
+    DEV void split(raw_t t, float mul, f16x8* f) { f[0] = mul < 0.f ? -t : t; }
 };
 template <> struct att_q<float> {
     static constexpr int N = 2;
-    DEV void load(const float* p, bool on, float sign, float mul, f16x8* f) {
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (on) {
-            io<float>::load(p, v);
-            io<float>::load(p + 4, v + 4);
-        }
+    struct raw_t {
+        f32x4 a, b;
+    };
+    DEV raw_t load(const float* p, bool on) {
+        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        return {on ? *(const f32x4*)p : z, on ? *(const f32x4*)(p + 4) : z};
+    }
+    DEV float absmax(raw_t t) {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) m = fmaxf(m, fmaxf(__builtin_fabsf(t.a[j]), __builtin_fabsf(t.b[j])));
+        return m;
+    }
+    DEV void split(raw_t t, float mul, f16x8* f) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float x = v[j] * (mul * sign);
+            const float x = (j < 4 ? t.a[j & 3] : t.b[j & 3]) * mul;
             f[0][j] = (f16_t)x;
             f[1][j] = (f16_t)(x - (float)f[0][j]);
         }
-    }
-    DEV float absmax(const float* p, bool on) {
-        float v[8], m = 0.f;
-        if (!on) return 0.f;
-        io<float>::load(p, v);
-        io<float>::load(p + 4, v + 4);
-#pragma unroll
-        for (int j = 0; j < 8; j++) m = fmaxf(m, __builtin_fabsf(v[j]));
-        return m;
     }
 };
 // The power of two that brings a row's largest magnitude to [2^13, 2^14), and its inverse; 1 for a row of zeros.
@@ -382,14 +377,15 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     const uint32_t hblocks = a.n_kv / a.heads, WK = W / a.heads;
     const uint32_t kvh = blockIdx.x % hblocks * a.heads + wave % a.heads, wk = wave / a.heads, piece = blockIdx.x / hblocks;
     uint64_t x0, x1, share;
-    const uint32_t all_tiles = att_share(a, piece, x0, x1, share);
+    att_line line;
+    const uint32_t all_tiles = att_share(a, piece, x0, x1, share, line);
     const bool lists = threadIdx.x == 0 && blockIdx.x % hblocks == 0 && a.scratch;
     if (lists && piece == 0) a.scratch[0] = a.list_tiles ? all_tiles : a.target;
     if (lists && !a.list_tiles) a.scratch[16 + 8 * piece + 3] = 0;  // no tile that goes on in the next piece, so far
     bool first_seg = true;
     for (uint64_t x = x0; x < x1; first_seg = false) {
     att_place it;
-    att_locate(a, x, it);
+    att_locate(a, x, line, it);
     const uint64_t tile_end = it.begin + it.s.umax, seg_end = min(tile_end, x1);
     const bool split = it.begin < x || tile_end > x1;
     const uint32_t slot = 2 * piece + (first_seg ? 0 : 1);
@@ -401,39 +397,29 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
             *(u32x4*)(d + 4) = u32x4{slot, 2 * (piece + 1), 2, 0};
         }
     }
-    const uint64_t flat_n = (uint64_t)it.s.m * a.group, flat0 = (uint64_t)it.tile * R;
-    const uint32_t rows_here = (uint32_t)min(flat_n - flat0, (uint64_t)R);
-    const uint32_t tok0 = (uint32_t)(flat0 / a.group), tok1 = (uint32_t)((flat0 + rows_here - 1) / a.group);
-    att_span sp = att_tile_span(a, it.s, 0, tok0, tok1);
+    const uint32_t flat_n = it.s.m * a.group, flat0 = it.tile * R, rows_here = min(flat_n - flat0, (uint32_t)R);
+    const uint32_t tok0 = flat0 / a.group, tok1 = (flat0 + rows_here - 1) / a.group;
+    att_span sp = att_tile_span<32>(a, it.s, tok0, tok1);
     sp.u1 = min(sp.u1, sp.u0 + (uint32_t)(seg_end - it.begin));
     sp.u0 = min(sp.u1, sp.u0 + (uint32_t)(x - it.begin));
     x = seg_end;
     const uint32_t* tab = a.table + (uint64_t)it.seq * a.max_pages;
-    const uint64_t kv_stride = (uint64_t)a.n_kv * HD;
+    const uint32_t kv_stride = a.n_kv * HD;
     const f16_t* kb = (const f16_t*)a.k + (uint64_t)kvh * HD;
     const f16_t* vb = (const f16_t*)a.v + (uint64_t)kvh * HD;
 
-    f16x8 qf[NB][KF][NQ];
+    typename att_q<T>::raw_t qr[NB][KF];
     float c[NB], m[NB], l[NB];
     int32_t pos[NB];
     uint64_t qat[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        const uint32_t flat = (uint32_t)flat0 + nb * 16 + n16, tok = flat / a.group;
+        const uint32_t flat = flat0 + nb * 16 + n16, tok = flat / a.group;
         const bool on = nb * 16 + n16 < rows_here;
         qat[nb] = on ? ((uint64_t)(it.s.row0 + tok) * a.n_q + kvh * a.group + flat % a.group) * HD : 0;
         pos[nb] = on ? it.s.p0 + (int32_t)tok : -1;
-        const T* qb = (const T*)a.q + qat[nb] + g * 8;
-        float mul = 1.f, inv = 1.f;
-        if constexpr (NQ == 2) {
-            float mx = 0.f;
 #pragma unroll
-            for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qb + s * 32, on));
-            att_q_scale(max_xor<32>(max_xor<16>(mx)), mul, inv);
-        }
-#pragma unroll
-        for (int s = 0; s < KF; s++) att_q<T>::load(qb + s * 32, on, a.sign, mul, qf[nb][s]);
-        c[nb] = a.c * inv;
+        for (int s = 0; s < KF; s++) qr[nb][s] = att_q<T>::load((const T*)a.q + qat[nb] + g * 8 + s * 32, on);
         m[nb] = NEG_INF;
         l[nb] = 0.f;
     }
@@ -482,6 +468,21 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
         load_k(row);
         __builtin_amdgcn_sched_barrier(0);
         load_v(row);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    f16x8 qf[NB][KF][NQ];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        float mul = 1.f, inv = 1.f;
+        if constexpr (NQ == 2) {
+            float mx = 0.f;
+#pragma unroll
+            for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qr[nb][s]));
+            att_q_scale(max_xor<32>(max_xor<16>(mx)), mul, inv);
+        }
+#pragma unroll
+        for (int s = 0; s < KF; s++) att_q<T>::split(qr[nb][s], mul * a.sign, qf[nb][s]);
+        c[nb] = a.c * inv;
     }
     while (key0 < k_end) {
         const int32_t next = key0 + stride;
@@ -669,7 +670,7 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
             }
         } else {
             const float inv = att_inverse(ls);
-            const uint32_t flat = (uint32_t)flat0 + r;
+            const uint32_t flat = flat0 + r;
             float t[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
             att_store4<T>((T*)a.out + ((uint64_t)(it.s.row0 + flat / a.group) * a.n_q + (kvh0 + h) * a.group + flat % a.group) * HD + col, t);
         }
@@ -715,19 +716,24 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
     att_item it;
     if (!att_find(a, blockIdx.x / H, it)) return;
     const uint32_t kvh = blockIdx.x % H;
-    const uint64_t flat_n = (uint64_t)it.s.m * a.group, flat0 = (uint64_t)it.tile * APK_ATT_CHUNK_ROWS;
-    const uint32_t tok0 = (uint32_t)(flat0 / a.group);
-    const uint32_t tok1 = (uint32_t)(min(flat0 + APK_ATT_CHUNK_ROWS, flat_n) - 1) / a.group;
-    const att_span sp = att_tile_span(a, it.s, it.part, tok0, tok1);
+    const uint32_t flat_n = it.s.m * a.group, flat0 = it.tile * APK_ATT_CHUNK_ROWS;
+    const uint32_t tok0 = flat0 / a.group, tok1 = (min(flat0 + APK_ATT_CHUNK_ROWS, flat_n) - 1) / a.group;
+    att_span sp = att_tile_span<BN>(a, it.s, tok0, tok1);
+    if (it.s.parts > 1) {
+        const uint64_t nu = sp.u1 - sp.u0;
+        const uint32_t first = sp.u0;
+        sp.u0 = first + (uint32_t)(nu * it.part / it.s.parts);
+        sp.u1 = first + (uint32_t)(nu * (it.part + 1) / it.s.parts);
+    }
     const uint32_t* tab = a.table + (uint64_t)it.seq * a.max_pages;
-    const uint64_t kv_stride = (uint64_t)a.n_kv * HD;
+    const uint32_t kv_stride = a.n_kv * HD;
     const f16_t* kb = (const f16_t*)a.k + (uint64_t)kvh * HD;
     const f16_t* vb = (const f16_t*)a.v + (uint64_t)kvh * HD;
 
     // this lane's row, and the first and last position of the wave's rows
-    const uint64_t flat = flat0 + wave * 32 + n32;
+    const uint32_t flat = flat0 + wave * 32 + n32;
     const bool on = flat < flat_n;
-    const uint32_t tok = (uint32_t)(flat / a.group), head = (uint32_t)(flat % a.group);
+    const uint32_t tok = flat / a.group, head = flat % a.group;
     const int32_t pos = on ? it.s.p0 + (int32_t)tok : -1;
     const int32_t pos_lo = a.window ? pos - (int32_t)a.window : -1;  // keys above this one
     const bool wave_on = flat0 + wave * 32 < flat_n;
@@ -739,16 +745,18 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
     f16x8 qf[KF][NQ];
     float c = a.c;
     {
-        const T* qb = (const T*)a.q + (on ? qat : 0);
+        typename att_q<T>::raw_t qr[KF];
         float mul = 1.f, inv = 1.f;
+#pragma unroll
+        for (int s = 0; s < KF; s++) qr[s] = att_q<T>::load((const T*)a.q + (on ? qat : 0) + s * 16 + hf * 8, on);
         if constexpr (NQ == 2) {
             float mx = 0.f;
 #pragma unroll
-            for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qb + s * 16 + hf * 8, on));
+            for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qr[s]));
             att_q_scale(max_xor<32>(mx), mul, inv);
         }
 #pragma unroll
-        for (int s = 0; s < KF; s++) att_q<T>::load(qb + s * 16 + hf * 8, on, a.sign, mul, qf[s]);
+        for (int s = 0; s < KF; s++) att_q<T>::split(qr[s], mul * a.sign, qf[s]);
         c *= inv;
     }
     f32x16 o[HB];
@@ -949,7 +957,7 @@ ATTEND_CHUNK(float, f32, 128, 64, 1)
 ATTEND_CHUNK(float, f32, 256, 32, 1)
 
 // ------------------------------------------------------------------------------------------- joining the parts
-// The tiles that were cut: a workgroup of eight waves takes join_rows (8 or 1) rows of one listed tile and kv head.  Of up
+// The tiles that were cut: a workgroup of eight waves takes join_rows rows of one listed tile and kv head.  Of up
 // to 32 parts a wave joins a row on its own, hd / 4 lanes to a part; of more the whole workgroup shares the parts of one
 // row after the other, so that the loads of all of them are under way together.
 template <typename T>
@@ -960,17 +968,17 @@ DEV void attend_join_body(const apk_attend_args& a) {
     if (j >= a.scratch[0]) return;
     const uint32_t* d = a.scratch + 16 + 8 * j;
     const uint32_t row0 = d[0], m = d[1], tile = d[2], parts = d[3], slot0 = d[4], slot1 = d[5], step = d[6];
-    const uint64_t flat0 = (uint64_t)tile * R + r0, flat_n = (uint64_t)m * a.group;
+    const uint32_t flat0 = tile * R + r0, flat_n = m * a.group;
     if (parts < 2 || flat0 >= flat_n) return;
-    const uint32_t rows = (uint32_t)min((uint64_t)a.join_rows, flat_n - flat0);
+    const uint32_t rows = min(a.join_rows, flat_n - flat0);
     const uint64_t to = (uint64_t)a.n_kv * R * (hd + 2);  // floats from slot to slot
     const float* base = att_part(a, 0, kvh);
     auto slot_of = [&](uint32_t p) { return base + (uint64_t)(p ? slot1 + (p - 1) * step : slot0) * to; };
     auto finish = [&](uint32_t r, uint32_t col, f32x4 t, float l) {
-        const uint64_t flat = flat0 + r;
+        const uint32_t flat = flat0 + r;
         const float inv = att_inverse(l);
         float v[4] = {t.x * inv, t.y * inv, t.z * inv, t.w * inv};
-        att_store4<T>((T*)a.out + ((uint64_t)(row0 + (uint32_t)(flat / a.group)) * a.n_q + kvh * a.group + (uint32_t)(flat % a.group)) * hd + col, v);
+        att_store4<T>((T*)a.out + ((uint64_t)(row0 + flat / a.group) * a.n_q + kvh * a.group + flat % a.group) * hd + col, v);
     };
     auto add = [](f32x4& acc, f32x4 v, float w) {
         acc.x = __builtin_fmaf(v.x, w, acc.x);
@@ -980,9 +988,8 @@ DEV void attend_join_body(const apk_attend_args& a) {
     };
     const uint32_t per = hd / 4, col = tid % per * 4;  // lanes of a part (16, 32 or 64)
     if (parts <= 32 && a.join_rows > 1) {
-        const uint32_t r = wave;
-        if (r >= rows) return;
         const uint32_t groups = 64 / per, grp = lane / per;
+        for (uint32_t r = wave; r < rows; r += 8) {
         float mp = NEG_INF, lp = 0.f;  // of part `lane`
         if (lane < parts) {
             const float* q = slot_of(lane) + (uint64_t)R * hd + r0 + r;
@@ -1014,6 +1021,7 @@ DEV void attend_join_body(const apk_attend_args& a) {
             acc.w += __shfl_xor(acc.w, g);
         }
         if (grp == 0) finish(r, col, acc, l);
+        }
         return;
     }
     const uint32_t groups = 512 / per, grp = tid / per;
@@ -1093,7 +1101,7 @@ DEV void attend_generic_body(const apk_attend_args& a, float* smem) {
     const int32_t pos = s.p0 + (int32_t)(row - s.row0);
     const int32_t hi = pos + 1, lo = a.window ? max(0, pos - (int32_t)a.window + 1) : 0;
     const uint32_t* tab = a.table + (uint64_t)seq * a.max_pages;
-    const uint64_t kv_stride = (uint64_t)a.n_kv * hd;
+    const uint32_t kv_stride = a.n_kv * hd;
     const f16_t* kb = (const f16_t*)a.k + (uint64_t)kvh * hd;
     const f16_t* vb = (const f16_t*)a.v + (uint64_t)kvh * hd;
     const uint64_t qat = ((uint64_t)row * a.n_q + h) * hd;
