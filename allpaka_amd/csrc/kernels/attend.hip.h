@@ -10,9 +10,12 @@
 // probabilities are already laid out as the second product's operand.  fp16 products are exact in f32.  With f32
 // activations a query element is the sum of two fp16 values (its row scaled by a power of two first), and so is a
 // probability: 22 bits of each take part.  With fp16 activations probabilities are rounded to fp16 once (an error of
-// 2^-12 relative at most, next to the 2^-12 of the fp16 result); they are held times 2^14, so that a key of weight down
-// to 2^-28 of the largest keeps all its bits, which a long cache of small weights needs.
+// 2^-11 relative at most, as that of the fp16 result).  Probabilities are 2^(x_j - r + 8), r a maximum met so far that is
+// replaced when one 2^7 times larger comes: they stay below 2^15, and a key of weight down to 2^-22 of r keeps all its bits,
+// which a long cache of small weights needs.
 #pragma once
+#include <type_traits>
+
 #include "../apk_attend.h"
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -20,7 +23,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-static constexpr float kProbShift = 14.0f;  // probabilities are held as 2^14 p
+static constexpr float kProbShift = 8.0f, kMaxLag = 7.0f;
 #define NEG_INF (-__builtin_inff())
 
 // {lane's own value, that of lane ^ X} in some order, X = 16 or 32: one swap of half rows, no LDS.  Written out, because
@@ -249,6 +252,19 @@ DEV void att_locate(const apk_attend_args& a, uint64_t x, att_line& ln, att_plac
     pl.number = rl(ln.tiles - ln.s.tiles, l) + pl.tile;
     pl.begin = first + (uint64_t)pl.tile * pl.s.umax;
 }
+// What is the same in all lanes, told to the compiler, which then keeps it in scalar registers and its branches uniform.
+DEV uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+DEV int32_t uni(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+DEV uint64_t uni(uint64_t v) { return ((uint64_t)uni((uint32_t)(v >> 32)) << 32) | uni((uint32_t)v); }
+DEV void uni_seq(att_seq& s) {
+    s.row0 = uni(s.row0);
+    s.m = uni(s.m);
+    s.n = uni(s.n);
+    s.p0 = uni(s.p0);
+    s.tiles = uni(s.tiles);
+    s.parts = uni(s.parts);
+    s.umax = uni(s.umax);
+}
 DEV float* att_part(const apk_attend_args& a, uint32_t slot, uint32_t kvh) {
     return (float*)((char*)a.scratch + APK_ATT_PART_AT) + ((uint64_t)slot * a.n_kv + kvh) * ((uint64_t)a.tile_rows * (a.hd + 2));
 }
@@ -379,6 +395,9 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     uint64_t x0, x1, share;
     att_line line;
     const uint32_t all_tiles = att_share(a, piece, x0, x1, share, line);
+    x0 = uni(x0);
+    x1 = uni(x1);
+    share = uni(share);
     const bool lists = threadIdx.x == 0 && blockIdx.x % hblocks == 0 && a.scratch;
     if (lists && piece == 0) a.scratch[0] = a.list_tiles ? all_tiles : a.target;
     if (lists && !a.list_tiles) a.scratch[16 + 8 * piece + 3] = 0;  // no tile that goes on in the next piece, so far
@@ -386,6 +405,11 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     for (uint64_t x = x0; x < x1; first_seg = false) {
     att_place it;
     att_locate(a, x, line, it);
+    it.seq = uni(it.seq);
+    it.tile = uni(it.tile);
+    it.number = uni(it.number);
+    it.begin = uni(it.begin);
+    uni_seq(it.s);
     const uint64_t tile_end = it.begin + it.s.umax, seg_end = min(tile_end, x1);
     const bool split = it.begin < x || tile_end > x1;
     const uint32_t slot = 2 * piece + (first_seg ? 0 : 1);
@@ -398,7 +422,7 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
         }
     }
     const uint32_t flat_n = it.s.m * a.group, flat0 = it.tile * R, rows_here = min(flat_n - flat0, (uint32_t)R);
-    const uint32_t tok0 = flat0 / a.group, tok1 = (flat0 + rows_here - 1) / a.group;
+    const uint32_t tok0 = uni(flat0 / a.group), tok1 = uni((flat0 + rows_here - 1) / a.group);
     att_span sp = att_tile_span<32>(a, it.s, tok0, tok1);
     sp.u1 = min(sp.u1, sp.u0 + (uint32_t)(seg_end - it.begin));
     sp.u0 = min(sp.u1, sp.u0 + (uint32_t)(x - it.begin));
@@ -520,15 +544,14 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
         for (int nb = 0; nb < NB; nb++) {
             float mx = fmaxf(fmaxf(fmaxf(s[nb][0][0], s[nb][0][1]), fmaxf(s[nb][0][2], s[nb][0][3])), fmaxf(fmaxf(s[nb][1][0], s[nb][1][1]), fmaxf(s[nb][1][2], s[nb][1][3])));
             mx = max_xor<32>(max_xor<16>(mx)) * c[nb];
-            const float mn = fmaxf(m[nb], mx), ms = mn == NEG_INF ? 0.f : mn;
-            if (__any(mn > m[nb])) {
-                const float alpha = exp2_hw(m[nb] - ms);
+            if (__any(mx > m[nb] + kMaxLag)) {  // the reference is moved on rarely: weights may grow to 2^kMaxLag
+                const float mn = fmaxf(m[nb], mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m[nb] - mn);
                 l[nb] *= alpha;
 #pragma unroll
                 for (int i = 0; i < CH; i++) o[nb][i] *= alpha;
                 m[nb] = mn;
             }
-            const float sub = kProbShift - ms;
+            const float sub = m[nb] == NEG_INF ? 0.f : kProbShift - m[nb];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float p = exp2_hw(__builtin_fmaf(s[nb][j >> 2][j & 3], c[nb], sub));
@@ -696,51 +719,89 @@ ATTEND_FEW(256, 1, 4)
 ATTEND_FEW(256, 2, 4)
 
 // ------------------------------------------------------------------------------------------- chunks of new tokens
-// One workgroup of four waves per (sequence, kv head, tile of 128 flat (token, head) rows, part of the keys).  Units of
-// BN keys go through LDS (fetched into registers while the unit before is worked on, two buffers, one barrier a unit); a
-// wave holds 32 rows.  K rows are the first operand of 32x32x16 products as they lie; V comes out of LDS transposed
-// (ds_read_b64_tr_b16), in the key order in which a lane holds its probabilities.  The 16-byte chunks of LDS row r are
-// permuted by f(r), so that both kinds of reads meet all banks.  Bound by the matrix and vector pipes together: for 32
-// rows x 32 keys x 128 channels 512 cycles of products stand next to about as many for the softmax.
+// One workgroup of four waves per (sequence, kv head, tile of 128 flat (token, head) rows, part of the keys); a wave holds 32
+// rows.  Units of BN keys go through LDS, written there by the loads themselves (no registers in between) into one of two
+// buffers while the unit in the other is worked on; one barrier a unit.  K rows are the first operand of 32x32x16 products
+// as they lie; V comes out of LDS transposed (ds_read_b64_tr_b16), in the key order in which a lane holds its
+// probabilities.  The 16-byte chunks of LDS row r are permuted by f(r), so that both kinds of reads meet all banks.
 template <int HD> DEV uint32_t att_swz(uint32_t r) {
     if constexpr (HD == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
     else return ((r & 3) << 2) | ((r >> 2) & 3);
 }
+typedef __attribute__((address_space(3))) char lds_t;
+// 16 bytes a lane from memory to LDS, lane l's to `at` + 16 l.  Counted by vmcnt like any load; the caller waits.
+DEV void lds_load16(const void* g, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(at) : "memory");
+}
+DEV void lds_arrived() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
 template <typename T, int HD, int BN>
-DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
+DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     constexpr int KF = HD / 16, NQ = att_q<T>::N, KB = BN / 32, HB = HD / 32, CPR = HD / 8;
     constexpr int NCH = BN * CPR / 256;  // 16-byte chunks of K (and of V) a thread stages
-    const uint32_t H = a.n_kv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n32 = lane & 31, hf = lane >> 5;
-    f16_t* const sk = smem;                    // [2][BN][HD]
-    f16_t* const sv = smem + 2 * BN * HD;      // [2][BN][HD]
+    constexpr uint32_t BUF = BN * HD * 2;  // bytes of a unit's K or V; K in buffers 0 and 1, V in 2 and 3
+    const uint32_t H = a.n_kv, tid = threadIdx.x, lane = tid & 63, n32 = lane & 31, hf = lane >> 5;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6);
+    lds_t* const lds = (lds_t*)smem;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
     att_item it;
     if (!att_find(a, blockIdx.x / H, it)) return;
+    it.seq = uni(it.seq);
+    it.tile = uni(it.tile);
+    it.part = uni(it.part);
+    it.slot = uni(it.slot);
+    uni_seq(it.s);
     const uint32_t kvh = blockIdx.x % H;
     const uint32_t flat_n = it.s.m * a.group, flat0 = it.tile * APK_ATT_CHUNK_ROWS;
-    const uint32_t tok0 = flat0 / a.group, tok1 = (min(flat0 + APK_ATT_CHUNK_ROWS, flat_n) - 1) / a.group;
+    const uint32_t tok0 = uni(flat0 / a.group), tok1 = uni((min(flat0 + APK_ATT_CHUNK_ROWS, flat_n) - 1) / a.group);
     att_span sp = att_tile_span<BN>(a, it.s, tok0, tok1);
     if (it.s.parts > 1) {
         const uint64_t nu = sp.u1 - sp.u0;
         const uint32_t first = sp.u0;
-        sp.u0 = first + (uint32_t)(nu * it.part / it.s.parts);
-        sp.u1 = first + (uint32_t)(nu * (it.part + 1) / it.s.parts);
+        sp.u0 = uni(first + (uint32_t)(nu * it.part / it.s.parts));
+        sp.u1 = uni(first + (uint32_t)(nu * (it.part + 1) / it.s.parts));
     }
     const uint32_t* tab = a.table + (uint64_t)it.seq * a.max_pages;
     const uint32_t kv_stride = a.n_kv * HD;
     const f16_t* kb = (const f16_t*)a.k + (uint64_t)kvh * HD;
     const f16_t* vb = (const f16_t*)a.v + (uint64_t)kvh * HD;
 
-    // this lane's row, and the first and last position of the wave's rows
+    // this lane's row, and the first and last position of the wave's and the tile's rows
     const uint32_t flat = flat0 + wave * 32 + n32;
     const bool on = flat < flat_n;
     const uint32_t tok = flat / a.group, head = flat % a.group;
     const int32_t pos = on ? it.s.p0 + (int32_t)tok : -1;
     const int32_t pos_lo = a.window ? pos - (int32_t)a.window : -1;  // keys above this one
     const bool wave_on = flat0 + wave * 32 < flat_n;
-    const int32_t wpos0 = it.s.p0 + (int32_t)((flat0 + wave * 32) / a.group);
-    const int32_t wpos1 = it.s.p0 + (int32_t)((min(flat0 + wave * 32 + 32, flat_n) - 1) / a.group);
+    const int32_t wpos0 = it.s.p0 + uni((int32_t)((flat0 + wave * 32) / a.group));
+    const int32_t wpos1 = it.s.p0 + uni((int32_t)((min(flat0 + wave * 32 + 32, flat_n) - 1) / a.group));
     const int32_t tpos0 = it.s.p0 + (int32_t)tok0, tpos1 = it.s.p0 + (int32_t)tok1;
     const uint64_t qat = ((uint64_t)(it.s.row0 + tok) * a.n_q + kvh * a.group + head) * HD;
+
+    // staging: thread t takes chunks t, t + 256, ... of a unit.  A lane looks one key up, a unit ahead; rows are handed round.
+    bool bad = false, odd = false;  // a table entry that names no page; a value of V that is not finite was cleared
+    att_entry ent;
+    auto look = [&](uint32_t u) { ent = att_look(a, tab, (int32_t)(u * BN + (lane & (BN - 1))), sp.lo, sp.hi); };
+    auto fetch = [&](uint32_t buf) {
+        const uint32_t row = att_row(a, ent, bad);
+#pragma unroll
+        for (int i = 0; i < NCH; i++) {
+            const uint32_t r = (i * 256 + tid) / CPR, ch = (tid % CPR) ^ att_swz<HD>(r);
+            const uint64_t at = (uint64_t)__shfl(row, r) * kv_stride + ch * 8;
+            const uint32_t to = lds0 + buf * BUF + (uint32_t)(i * 256 + wave * 64) * 16;
+            lds_load16(kb + at, to);
+            lds_load16(vb + at, to + 2 * BUF);
+        }
+    };
+    // some row of the tile does not see all keys of this unit
+    auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
+    if (sp.u0 < sp.u1) {
+        look(sp.u0);
+        fetch(0);
+        look(sp.u0 + 1);
+    }
 
     f16x8 qf[KF][NQ];
     float c = a.c;
@@ -765,79 +826,71 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
     float m = NEG_INF, l = 0.f;
+    // where this lane finds its fragments: K chunk 2 i + hf of row n32 (+ 32 b); V channels 32 hb + .. of four keys
+    uint32_t ka[KF], va[HB][2];
+#pragma unroll
+    for (int i = 0; i < KF; i++) ka[i] = n32 * (HD * 2) + (((i * 2 + hf) ^ att_swz<HD>(n32)) * 16);
+#pragma unroll
+    for (int hb = 0; hb < HB; hb++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t r = e * 8 + hf * 4 + ((lane & 15) >> 2), ch = hb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+            va[hb][e] = r * (HD * 2) + ((ch ^ att_swz<HD>(r)) * 16) + (lane & 1) * 8;
+        }
+    lds_arrived();
 
-    // some row of the tile does not see all keys of this unit
-    auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
-    bool odd = false;  // a value of V that is not finite was cleared
-    // staging: thread t takes chunks t, t + 256, ... of a unit
-    att_entry ent[NCH];
-    bool bad = false;
-    u32x4 rk[NCH], rv[NCH];
-    auto look = [&](uint32_t u) {
-#pragma unroll
-        for (int i = 0; i < NCH; i++) ent[i] = att_look(a, tab, (int32_t)(u * BN + (i * 256 + tid) / CPR), sp.lo, sp.hi);
-    };
-    auto fetch = [&]() {
-#pragma unroll
-        for (int i = 0; i < NCH; i++) {
-            const uint32_t p = i * 256 + tid, r = p / CPR, ch = (p % CPR) ^ att_swz<HD>(r);
-            const uint64_t at = (uint64_t)att_row(a, ent[i], bad) * kv_stride + ch * 8;
-            rk[i] = *(const u32x4*)(kb + at);
-            rv[i] = *(const u32x4*)(vb + at);
-        }
-    };
-    auto stage = [&](uint32_t u) {
+    // (a wave without rows only stages; all others work on every unit: a condition here costs copies of the outputs)
+    auto work = [&](uint32_t u, auto buf_, auto on_) {
+        constexpr uint32_t buf = decltype(buf_)::value;
+        constexpr bool with_rows = decltype(on_)::value;
+        fetch(1 - buf);  // (behind the last unit: row 0, not used; a condition would make the compiler wait for the entries)
+        look(u + 2);
         const int32_t key0 = (int32_t)(u * BN);
-        const bool edge = key0 < sp.lo || key0 + BN > sp.hi;
-        const bool partial = is_partial(key0);
-        f16_t* dk = sk + (u & 1) * (BN * HD);
-        f16_t* dv = sv + (u & 1) * (BN * HD);
-#pragma unroll
-        for (int i = 0; i < NCH; i++) {
-            const uint32_t p = i * 256 + tid;
-            if (edge) {
+        if (key0 < sp.lo || is_partial(key0)) {
+            // keys that no row sees are cleared in V, so that what lies there meets no weight of zero; so are values that
+            // are not finite, which the rows that see them get at the end
+#pragma unroll 1
+            for (int i = 0; i < NCH; i++) {
+                const uint32_t p = i * 256 + tid;
                 const int32_t key = key0 + (int32_t)(p / CPR);
-                if (key < sp.lo || key >= sp.hi) rv[i] = u32x4{0u, 0u, 0u, 0u};
-            }
-            if (partial && att_nonfinite(rv[i])) {
-                odd = true;
-                rv[i] = att_clear_nonfinite(rv[i]);
-            }
-            *(u32x4*)(dk + p * 8) = rk[i];
-            *(u32x4*)(dv + p * 8) = rv[i];
-        }
-    };
-    if (sp.u0 < sp.u1) {
-        look(sp.u0);
-        fetch();
-        if (sp.u0 + 1 < sp.u1) look(sp.u0 + 1);
-        stage(sp.u0);
-    }
-    __syncthreads();
-    for (uint32_t u = sp.u0; u < sp.u1; u++) {
-        if (u + 1 < sp.u1) {
-            fetch();
-            if (u + 2 < sp.u1) look(u + 2);
-        }
-        const f16_t* tk = sk + (u & 1) * (BN * HD);
-        const f16_t* tv = sv + (u & 1) * (BN * HD);
-        const int32_t key0 = (int32_t)(u * BN);
-        const bool active = wave_on && key0 <= wpos1 && (!a.window || key0 + BN - 1 > wpos0 - (int32_t)a.window);
-        f16x8 ph[KB][2], pl[KB][2];
-        if (active) {
-            f32x16 s[KB];
-#pragma unroll
-            for (int b = 0; b < KB; b++) {
-#pragma unroll
-                for (int j = 0; j < 16; j++) s[b][j] = 0.f;
-                const uint32_t r = b * 32 + n32;
-#pragma unroll
-                for (int i = 0; i < KF; i++) {
-                    const f16x8 kf = *(const f16x8*)(tk + r * HD + (((i * 2 + hf) ^ att_swz<HD>(r)) * 8));
-#pragma unroll
-                    for (int t = 0; t < NQ; t++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i][t], s[b], 0, 0, 0);
+                __attribute__((address_space(3))) u32x4* at = (__attribute__((address_space(3))) u32x4*)(lds + (2 + buf) * BUF + p * 16);
+                if (key < sp.lo || key >= sp.hi) {
+                    *at = u32x4{0u, 0u, 0u, 0u};
+                } else {
+                    const u32x4 t = *at;
+                    if (att_nonfinite(t)) {
+                        odd = true;
+                        *at = att_clear_nonfinite(t);
+                    }
                 }
             }
+            __syncthreads();
+        }
+        if constexpr (with_rows) {
+            f32x16 s[KB];
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[b][j] = 0.f;
+            f16x8 kf[KB][KF];
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int i = 0; i < KF; i++) kf[b][i] = *(__attribute__((address_space(3))) f16x8*)(lds + (ka[i] + buf * BUF + b * 32 * HD * 2));
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int i = 0; i < KF; i++)
+#pragma unroll
+                    for (int t = 0; t < NQ; t++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b][i], qf[i][t], s[b], 0, 0, 0);
+            // the first fragments, then one more for every product
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < KB * KF - 4; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4 * NQ, 0);
             if (key0 + BN - 1 > wpos0 || (a.window && key0 <= wpos1 - (int32_t)a.window)) {
 #pragma unroll
                 for (int b = 0; b < KB; b++)
@@ -853,15 +906,15 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
 #pragma unroll
                 for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
             mx = max_xor<32>(mx) * c;
-            const float mn = fmaxf(m, mx), ms = mn == NEG_INF ? 0.f : mn;
-            if (__any(mn > m)) {
-                const float alpha = exp2_hw(m - ms);
+            if (__any(mx > m + kMaxLag)) {  // the reference is moved on rarely: weights may grow to 2^kMaxLag
+                const float mn = fmaxf(m, mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
                 l *= alpha;
 #pragma unroll
                 for (int i = 0; i < HB; i++) o[i] *= alpha;
                 m = mn;
             }
-            const float sub = kProbShift - ms;
+            const float sub = m == NEG_INF ? 0.f : kProbShift - m;
+            f16x8 ph[KB][2], pl[KB][2];
 #pragma unroll
             for (int b = 0; b < KB; b++)
 #pragma unroll
@@ -872,11 +925,8 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
                     ph[b][j >> 3][j & 7] = h;
                     if constexpr (NQ == 2) pl[b][j >> 3][j & 7] = (f16_t)(p - (float)h);
                 }
-        }
-        if (active) {
-            const uint32_t l16 = lane & 15, half = (lane >> 4) & 1;
-#pragma unroll
-            for (int hb = 0; hb < HB; hb++)
+            // fragments of 32 channels at a time, the next ones under way
+            auto load_v = [&](int hb, f16x8* vf) {
 #pragma unroll
                 for (int b = 0; b < KB; b++)
 #pragma unroll
@@ -884,32 +934,60 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
                         union {
                             s16x4 h[2];
                             f16x8 v;
-                        } vf;
+                        } t;
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const uint32_t r = b * 32 + q * 16 + e * 8 + hf * 4 + (l16 >> 2);
-                            const uint32_t ch = hb * 4 + half * 2 + ((l16 & 3) >> 1);
-                            const f16_t* p = tv + r * HD + ((ch ^ att_swz<HD>(r)) * 8) + (l16 & 1) * 4;
-                            vf.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-                        }
-                        o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.v, ph[b][q], o[hb], 0, 0, 0);
-                        if constexpr (NQ == 2) o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.v, pl[b][q], o[hb], 0, 0, 0);
+                        for (int e = 0; e < 2; e++)
+                            t.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4*)(lds + (va[hb][e] + (2 + buf) * BUF + (b * 32 + q * 16) * HD * 2)));
+                        vf[b * 2 + q] = t.v;
                     }
+            };
+            f16x8 vf[2][2 * KB];
+            load_v(0, vf[0]);
+#pragma unroll
+            for (int hb = 0; hb < HB; hb++) {
+                if (hb + 1 < HB) load_v(hb + 1, vf[(hb + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 2 * KB; k++) {
+                    o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[hb & 1][k], ph[k >> 1][k & 1], o[hb], 0, 0, 0);
+                    if constexpr (NQ == 2) o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[hb & 1][k], pl[k >> 1][k & 1], o[hb], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        if (u + 1 < sp.u1) stage(u + 1);
-        __syncthreads();
+        lds_arrived();
+    };
+    constexpr std::integral_constant<uint32_t, 0> b0;
+    constexpr std::integral_constant<uint32_t, 1> b1;
+    if (wave_on) {
+        for (uint32_t u = sp.u0; u < sp.u1; u++) {
+            work(u, b0, std::true_type());
+            if (++u >= sp.u1) break;
+            work(u, b1, std::true_type());
+        }
+    } else {
+#pragma unroll 1
+        for (uint32_t u = sp.u0; u < sp.u1; u++) {
+            work(u, b0, std::false_type());
+            if (++u >= sp.u1) break;
+            work(u, b1, std::false_type());
+        }
     }
     att_report(a, bad);
-    // A value of V that is not finite, in a unit that some rows see only in part, was cleared on its way in, so that it
-    // met no weight of zero; the rows that do see it get it here, as it is (any weight above zero leaves it so).
-    if (__syncthreads_or(odd)) {
+    if (tid == 0) *(__attribute__((address_space(3))) uint32_t*)lds = 0;
+    __syncthreads();
+    if (odd) *(__attribute__((address_space(3))) uint32_t*)lds = 1;
+    __syncthreads();
+    if (*(__attribute__((address_space(3))) uint32_t*)lds) {
 #pragma unroll 1
         for (uint32_t u = sp.u0; u < sp.u1; u++) {
             if (!is_partial((int32_t)(u * BN))) continue;
 #pragma unroll 1
             for (int32_t key = (int32_t)(u * BN); key < (int32_t)(u * BN) + BN; key++) {
                 if (key < sp.lo || key > pos || (a.window && key <= pos_lo)) continue;
-                const f16_t* p = vb + (uint64_t)att_row(a, att_look(a, tab, key, sp.lo, sp.hi), bad) * kv_stride + 4 * hf;
+                bool no = false;
+                const f16_t* p = vb + (uint64_t)att_row(a, att_look(a, tab, key, sp.lo, sp.hi), no) * kv_stride + 4 * hf;
 #pragma unroll
                 for (int hb = 0; hb < HB; hb++)
 #pragma unroll
@@ -948,7 +1026,10 @@ DEV void attend_chunk_body(const apk_attend_args& a, f16_t* smem) {
             att_store4<T>(out + hb * 32 + 8 * (j >> 2) + 4 * hf, t);
         }
 }
-#define ATTEND_CHUNK(T, t, HD, BN, WPE)                                                                              extern "C" __global__ __launch_bounds__(256, WPE) void apk_attend_chunk_##t##_hd##HD(apk_attend_args a) {            attend_chunk_body<T, HD, BN>(a, (f16_t*)att_smem);                                                           }
+#define ATTEND_CHUNK(T, t, HD, BN, WPE)                                                                          \
+    extern "C" __global__ __launch_bounds__(256, WPE) void apk_attend_chunk_##t##_hd##HD(apk_attend_args a) {    \
+        attend_chunk_body<T, HD, BN>(a, (char*)att_smem);                                                        \
+    }
 ATTEND_CHUNK(f16_t, f16, 64, 64, 2)
 ATTEND_CHUNK(f16_t, f16, 128, 64, 2)
 ATTEND_CHUNK(f16_t, f16, 256, 32, 1)
