@@ -15,6 +15,7 @@
 // which a long cache of small weights needs.
 #pragma once
 #include <type_traits>
+#include <utility>
 
 #include "../apk_attend.h"
 
@@ -729,6 +730,10 @@ template <int HD> DEV uint32_t att_swz(uint32_t r) {
     else return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 typedef __attribute__((address_space(3))) char lds_t;
+template <typename F, int... I> DEV void static_for_(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }
+template <int N, typename F> DEV void static_for(F&& f) { static_for_(f, std::make_integer_sequence<int, N>()); }
+// The value of lane J of this lane's run of 16.
+template <int J> DEV uint32_t run_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x150 + J, 0xf, 0xf, true); }
 // 16 bytes a lane from memory to LDS, lane l's to `at` + 16 l.  Counted by vmcnt like any load; the caller waits.
 DEV void lds_load16(const void* g, uint32_t at) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(at) : "memory");
@@ -782,27 +787,33 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
 
     // staging: thread t takes chunks t, t + 256, ... of a unit.  A lane looks one key up, a unit ahead; rows are handed round.
     bool bad = false, odd = false;  // a table entry that names no page; a value of V that is not finite was cleared
+    // (thread t's chunk i is one of row (256 i + t) / CPR.  In a run of 16 lanes lane j < NCH * RPR looks up the row that
+    // chunk j % NCH of the lanes 16 / RPR * (j / NCH) .. needs, and hands it to them.)
+    constexpr int RPR = CPR < 16 ? 16 / CPR : 1;  // rows that 16 lanes touch
+    static_assert(NCH * RPR <= 16, "rows of a run of lanes");
     att_entry ent;
-    auto look = [&](uint32_t u) { ent = att_look(a, tab, (int32_t)(u * BN + (lane & (BN - 1))), sp.lo, sp.hi); };
+    auto look = [&](uint32_t u) {
+        const uint32_t j = lane & 15, i = j % NCH, h = j / NCH % RPR;
+        ent = att_look(a, tab, (int32_t)(u * BN + (i * 256 + (tid & ~15u)) / CPR + h), sp.lo, sp.hi);
+    };
     auto fetch = [&](uint32_t buf) {
         const uint32_t row = att_row(a, ent, bad);
-#pragma unroll
-        for (int i = 0; i < NCH; i++) {
+        const uint32_t to = lds0 + buf * BUF + wave * 1024;
+        static_for<NCH>([&](auto i_) {
+            constexpr int i = decltype(i_)::value;
             const uint32_t r = (i * 256 + tid) / CPR, ch = (tid % CPR) ^ att_swz<HD>(r);
-            const uint64_t at = (uint64_t)__shfl(row, r) * kv_stride + ch * 8;
-            const uint32_t to = lds0 + buf * BUF + (uint32_t)(i * 256 + wave * 64) * 16;
-            lds_load16(kb + at, to);
-            lds_load16(vb + at, to + 2 * BUF);
-        }
+            uint32_t from = run_lane<i>(row);
+            if constexpr (RPR == 2) {  // (both read by all lanes: a lane that is off hands nothing on)
+                const uint32_t other = run_lane<NCH + i>(row);
+                from = (lane & 8) ? other : from;
+            }
+            const uint64_t at = (uint64_t)from * kv_stride + ch * 8;
+            lds_load16(kb + at, to + i * 4096);
+            lds_load16(vb + at, to + i * 4096 + 2 * BUF);
+        });
     };
     // some row of the tile does not see all keys of this unit
     auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
-    if (sp.u0 < sp.u1) {
-        look(sp.u0);
-        fetch(0);
-        look(sp.u0 + 1);
-    }
-
     f16x8 qf[KF][NQ];
     float c = a.c;
     {
@@ -837,18 +848,151 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             const uint32_t r = e * 8 + hf * 4 + ((lane & 15) >> 2), ch = hb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
             va[hb][e] = r * (HD * 2) + ((ch ^ att_swz<HD>(r)) * 16) + (lane & 1) * 8;
         }
-    lds_arrived();
 
-    // (a wave without rows only stages; all others work on every unit: a condition here costs copies of the outputs)
-    auto work = [&](uint32_t u, auto buf_, auto on_) {
-        constexpr uint32_t buf = decltype(buf_)::value;
-        constexpr bool with_rows = decltype(on_)::value;
-        fetch(1 - buf);  // (behind the last unit: row 0, not used; a condition would make the compiler wait for the entries)
+    f32x16 s[KB];
+    f16x8 ph[KB][2], pl[KB][2];
+    auto load_k = [&](int b, int i, uint32_t k_at) { return *(__attribute__((address_space(3))) f16x8*)(lds + (ka[i] + k_at + b * 32 * HD * 2)); };
+    auto score = [&](int b, int i, f16x8 kf) {
+        if (i == 0) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[b][j] = 0.f;
+        }
+#pragma unroll
+        for (int t = 0; t < NQ; t++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i][t], s[b], 0, 0, 0);
+    };
+    // 16 keys of 32 channels, transposed.  (The compiler neither moves these reads nor lets others pass them: where they
+    // stand is where they are issued.)
+    auto load_v = [&](int hb, int b, int q, uint32_t v_at) {
+        union {
+            s16x4 h[2];
+            f16x8 v;
+        } t;
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            t.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + (va[hb][e] + v_at + (b * 32 + q * 16) * HD * 2)));
+        return t.v;
+    };
+    auto value = [&](int hb, int b, int q, f16x8 vf) {
+        o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b][q], o[hb], 0, 0, 0);
+        if constexpr (NQ == 2) o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b][q], o[hb], 0, 0, 0);
+    };
+    auto weight = [&](int b, int j, float sub) {
+        const float p = exp2_hw(__builtin_fmaf(s[b][j], c, sub));
+        l += p;
+        const f16_t h = (f16_t)p;
+        ph[b][j >> 3][j & 7] = h;
+        if constexpr (NQ == 2) pl[b][j >> 3][j & 7] = (f16_t)(p - (float)h);
+    };
+    auto shift = [&]() { return m == NEG_INF ? 0.f : kProbShift - m; };
+    auto values = [&](int b, uint32_t v_at) {
+        f16x8 vf[2][2];
+#pragma unroll
+        for (int q = 0; q < 2; q++) vf[0][q] = load_v(0, b, q, v_at);
+#pragma unroll
+        for (int hb = 0; hb < HB; hb++) {
+            if (hb + 1 < HB) {
+#pragma unroll
+                for (int q = 0; q < 2; q++) vf[(hb + 1) & 1][q] = load_v(hb + 1, b, q, v_at);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int q = 0; q < 2; q++) value(hb, b, q, vf[hb & 1][q]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // moves the reference on where a block's maximum asks for it; `before` runs first: products of weights that refer to
+    // the old one
+    auto refer = [&](int b, auto&& before) {
+        float mx = NEG_INF;
+#pragma unroll
+        for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
+        mx = max_xor<32>(mx) * c;
+        if (__any(mx > m + kMaxLag)) {
+            before();
+            const float mn = fmaxf(m, mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < HB; i++) o[i] *= alpha;
+            m = mn;
+        }
+    };
+    // A unit that all rows see whole, in buffer `buf`.  Blocks of 32 keys, so that a wave has products and softmax to run
+    // side by side: the products of block 1's scores next to block 0's exponentials, those of block 0's values next to
+    // block 1's; LDS reads stand a few products before their use.  (fetch: behind the last unit it reads row 0, which is
+    // not used; a condition would make the compiler wait for the table entries.)
+    auto whole = [&](uint32_t u, auto buf_) {
+        constexpr uint32_t buf = decltype(buf_)::value, k_at = buf * BUF, v_at = (2 + buf) * BUF;
+        constexpr int AHEAD = KF < 4 ? KF : 4;  // fragments read ahead
+        f16x8 kf[KF];
+#pragma unroll
+        for (int i = 0; i < KF; i++) kf[i] = load_k(0, i, k_at);
+#pragma unroll
+        for (int i = 0; i < KF; i++) score(0, i, kf[i]);
+        fetch(1 - buf);
+        look(u + 2);
+        if constexpr (KB == 2) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) kf[i] = load_k(1, i, k_at);
+            refer(0, [] {});
+            float sub = shift();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < KF; i++) {
+                if (i + AHEAD < KF) kf[i + AHEAD] = load_k(1, i + AHEAD, k_at);
+                score(1, i, kf[i]);
+#pragma unroll
+                for (int j = i * 16 / KF; j < (i + 1) * 16 / KF; j++) weight(0, j, sub);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            f16x8 vf[2][2];
+#pragma unroll
+            for (int q = 0; q < 2; q++) vf[0][q] = load_v(0, 0, q, v_at);
+            refer(1, [&] {
+                values(0, v_at);
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    ph[0][q] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+                    if constexpr (NQ == 2) pl[0][q] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+                }
+            });
+            sub = shift();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2 * HB; k++) {  // block 0's values, then block 1's
+                const int hb = k % HB, b = k / HB, nhb = (k + 1) % HB, nb = (k + 1) / HB;
+                if (k + 1 < 2 * HB) {
+#pragma unroll
+                    for (int q = 0; q < 2; q++) vf[(k + 1) & 1][q] = load_v(nhb, nb, q, v_at);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    value(hb, b, q, vf[k & 1][q]);
+                    if (b == 0) {
+                        const int x = hb * 2 + q;
+#pragma unroll
+                        for (int j = x * 16 / (2 * HB); j < (x + 1) * 16 / (2 * HB); j++) weight(1, j, sub);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            refer(0, [] {});
+            const float sub = shift();
+#pragma unroll
+            for (int j = 0; j < 16; j++) weight(0, j, sub);
+            values(0, v_at);
+        }
+        lds_arrived();
+    };
+    // Any unit: rows that do not see all of it have scores of -inf.  Keys that no row sees are cleared in V, so that what
+    // lies there meets no weight of zero; so are values that are not finite, which the rows that see them get at the end.
+    auto part_seen = [&](uint32_t u, uint32_t buf) {
+        fetch(1 - buf);
         look(u + 2);
         const int32_t key0 = (int32_t)(u * BN);
         if (key0 < sp.lo || is_partial(key0)) {
-            // keys that no row sees are cleared in V, so that what lies there meets no weight of zero; so are values that
-            // are not finite, which the rows that see them get at the end
 #pragma unroll 1
             for (int i = 0; i < NCH; i++) {
                 const uint32_t p = i * 256 + tid;
@@ -866,113 +1010,48 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             }
             __syncthreads();
         }
-        if constexpr (with_rows) {
-            f32x16 s[KB];
+        if (wave_on && key0 <= wpos1 && (!a.window || key0 + BN - 1 > wpos0 - (int32_t)a.window)) {
 #pragma unroll
-            for (int b = 0; b < KB; b++)
+            for (int b = 0; b < KB; b++) {
 #pragma unroll
-                for (int j = 0; j < 16; j++) s[b][j] = 0.f;
-            f16x8 kf[KB][KF];
-#pragma unroll
-            for (int b = 0; b < KB; b++)
-#pragma unroll
-                for (int i = 0; i < KF; i++) kf[b][i] = *(__attribute__((address_space(3))) f16x8*)(lds + (ka[i] + buf * BUF + b * 32 * HD * 2));
-#pragma unroll
-            for (int b = 0; b < KB; b++)
-#pragma unroll
-                for (int i = 0; i < KF; i++)
-#pragma unroll
-                    for (int t = 0; t < NQ; t++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b][i], qf[i][t], s[b], 0, 0, 0);
-            // the first fragments, then one more for every product
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-            for (int i = 0; i < KB * KF - 4; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, 4 * NQ, 0);
-            if (key0 + BN - 1 > wpos0 || (a.window && key0 <= wpos1 - (int32_t)a.window)) {
-#pragma unroll
-                for (int b = 0; b < KB; b++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int32_t key = key0 + b * 32 + 8 * (j >> 2) + 4 * (int32_t)hf + (j & 3);
-                        if (key > pos || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
-                    }
-            }
-            float mx = NEG_INF;
-#pragma unroll
-            for (int b = 0; b < KB; b++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
-            mx = max_xor<32>(mx) * c;
-            if (__any(mx > m + kMaxLag)) {  // the reference is moved on rarely: weights may grow to 2^kMaxLag
-                const float mn = fmaxf(m, mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
-                l *= alpha;
-#pragma unroll
-                for (int i = 0; i < HB; i++) o[i] *= alpha;
-                m = mn;
-            }
-            const float sub = m == NEG_INF ? 0.f : kProbShift - m;
-            f16x8 ph[KB][2], pl[KB][2];
-#pragma unroll
-            for (int b = 0; b < KB; b++)
+                for (int i = 0; i < KF; i++) score(b, i, load_k(b, i, buf * BUF));
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const float p = exp2_hw(__builtin_fmaf(s[b][j], c, sub));
-                    l += p;
-                    const f16_t h = (f16_t)p;
-                    ph[b][j >> 3][j & 7] = h;
-                    if constexpr (NQ == 2) pl[b][j >> 3][j & 7] = (f16_t)(p - (float)h);
+                    const int32_t key = key0 + b * 32 + 8 * (j >> 2) + 4 * (int32_t)hf + (j & 3);
+                    if (key > pos || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
                 }
-            // fragments of 32 channels at a time, the next ones under way
-            auto load_v = [&](int hb, f16x8* vf) {
+                refer(b, [] {});
+                const float sub = shift();
 #pragma unroll
-                for (int b = 0; b < KB; b++)
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        union {
-                            s16x4 h[2];
-                            f16x8 v;
-                        } t;
-#pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            t.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4*)(lds + (va[hb][e] + (2 + buf) * BUF + (b * 32 + q * 16) * HD * 2)));
-                        vf[b * 2 + q] = t.v;
-                    }
-            };
-            f16x8 vf[2][2 * KB];
-            load_v(0, vf[0]);
-#pragma unroll
-            for (int hb = 0; hb < HB; hb++) {
-                if (hb + 1 < HB) load_v(hb + 1, vf[(hb + 1) & 1]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int k = 0; k < 2 * KB; k++) {
-                    o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[hb & 1][k], ph[k >> 1][k & 1], o[hb], 0, 0, 0);
-                    if constexpr (NQ == 2) o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[hb & 1][k], pl[k >> 1][k & 1], o[hb], 0, 0, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < 16; j++) weight(b, j, sub);
+                values(b, (2 + buf) * BUF);
             }
         }
         lds_arrived();
     };
-    constexpr std::integral_constant<uint32_t, 0> b0;
-    constexpr std::integral_constant<uint32_t, 1> b1;
-    if (wave_on) {
-        for (uint32_t u = sp.u0; u < sp.u1; u++) {
-            work(u, b0, std::true_type());
-            if (++u >= sp.u1) break;
-            work(u, b1, std::true_type());
-        }
-    } else {
+    // units [f0, f1), an even number, are seen whole by all rows
+    int32_t w0 = a.window ? tpos1 - (int32_t)a.window + 1 : 0, w1 = tpos0 + 1;
+    uint32_t f0 = max(sp.u0, (uint32_t)max(0, (max(w0, sp.lo) + BN - 1) / BN)), f1 = min(sp.u1, (uint32_t)max(0, w1 / BN));
+    f0 = min(f0, sp.u1);
+    f1 = f1 > f0 && wave_on ? f0 + ((f1 - f0) & ~1u) : f0;
+    const uint32_t parity = f0 & 1;
+    if (sp.u0 < sp.u1) {
+        look(sp.u0);
+        fetch((sp.u0 ^ parity) & 1);
+        look(sp.u0 + 1);
+    }
+    lds_arrived();
+    uint32_t u = sp.u0, stop = f0;
 #pragma unroll 1
-        for (uint32_t u = sp.u0; u < sp.u1; u++) {
-            work(u, b0, std::false_type());
-            if (++u >= sp.u1) break;
-            work(u, b1, std::false_type());
+    for (;;) {
+#pragma unroll 1
+        for (; u < stop; u++) part_seen(u, (u ^ parity) & 1);
+        if (u >= sp.u1) break;
+        for (; u < f1; u += 2) {
+            whole(u, std::integral_constant<uint32_t, 0>());
+            whole(u + 1, std::integral_constant<uint32_t, 1>());
         }
+        stop = sp.u1;
     }
     att_report(a, bad);
     if (tid == 0) *(__attribute__((address_space(3))) uint32_t*)lds = 0;
