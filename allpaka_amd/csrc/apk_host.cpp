@@ -1662,7 +1662,7 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
         kernel = "apk_attend_few_" + t_name + "_hd" + std::to_string(head_dim) + "_b" + std::to_string(nb);
     } else {
         a.tile_rows = APK_ATT_CHUNK_ROWS;
-        a.unit = head_dim == 256 ? 32 : 64;
+        a.unit = 64;
         a.heads = 1;
         a.target = 512;
         a.unit_min = 512 / a.unit;

@@ -900,65 +900,102 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // moves the reference on where a block's maximum asks for it; `before` runs first: products of weights that refer to
-    // the old one
-    auto refer = [&](int b, auto&& before) {
+    // moves the reference on where a block's maximum asks for it; `again` redoes weights that refer to the old one
+    auto refer = [&](int b, auto&& again) {
         float mx = NEG_INF;
 #pragma unroll
         for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
         mx = max_xor<32>(mx) * c;
         if (__any(mx > m + kMaxLag)) {
-            before();
             const float mn = fmaxf(m, mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
-            l *= alpha;
+            m = mn;
+            again(alpha);
 #pragma unroll
             for (int i = 0; i < HB; i++) o[i] *= alpha;
-            m = mn;
+        }
+    };
+    // Keys that no row sees are cleared in V, so that what lies there meets no weight of zero; so are values that are not
+    // finite, which the rows that see them get at the end.
+    auto clear = [&](int32_t key0, uint32_t buf) {
+#pragma unroll 1
+        for (int i = 0; i < NCH; i++) {
+            const uint32_t p = i * 256 + tid;
+            const int32_t key = key0 + (int32_t)(p / CPR);
+            __attribute__((address_space(3))) u32x4* at = (__attribute__((address_space(3))) u32x4*)(lds + (2 + buf) * BUF + p * 16);
+            if (key < sp.lo || key >= sp.hi) {
+                *at = u32x4{0u, 0u, 0u, 0u};
+            } else {
+                const u32x4 t = *at;
+                if (att_nonfinite(t)) {
+                    odd = true;
+                    *at = att_clear_nonfinite(t);
+                }
+            }
+        }
+        __syncthreads();
+    };
+    auto hide = [&](int b, int32_t key0) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int32_t key = key0 + b * 32 + 8 * (j >> 2) + 4 * (int32_t)hf + (j & 3);
+            if (key > pos || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
         }
     };
     // A unit that all rows see whole, in buffer `buf`.  Blocks of 32 keys, so that a wave has products and softmax to run
     // side by side: the products of block 1's scores next to block 0's exponentials, those of block 0's values next to
     // block 1's; LDS reads stand a few products before their use.  (fetch: behind the last unit it reads row 0, which is
     // not used; a condition would make the compiler wait for the table entries.)
-    auto whole = [&](uint32_t u, auto buf_) {
+    auto whole = [&](uint32_t u, auto buf_, auto any_) {
+        constexpr bool ANY = decltype(any_)::value;
+        const int32_t key0 = (int32_t)(u * BN);
+        const bool partial = ANY && (key0 < sp.lo || is_partial(key0));
         constexpr uint32_t buf = decltype(buf_)::value, k_at = buf * BUF, v_at = (2 + buf) * BUF;
         constexpr int AHEAD = KF < 4 ? KF : 4;  // fragments read ahead
         f16x8 kf[KF];
 #pragma unroll
-        for (int i = 0; i < KF; i++) kf[i] = load_k(0, i, k_at);
-#pragma unroll
-        for (int i = 0; i < KF; i++) score(0, i, kf[i]);
-        fetch(1 - buf);
-        look(u + 2);
-        if constexpr (KB == 2) {
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++) kf[i] = load_k(1, i, k_at);
-            refer(0, [] {});
-            float sub = shift();
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < KF; i++) {
-                if (i + AHEAD < KF) kf[i + AHEAD] = load_k(1, i + AHEAD, k_at);
-                score(1, i, kf[i]);
-#pragma unroll
-                for (int j = i * 16 / KF; j < (i + 1) * 16 / KF; j++) weight(0, j, sub);
+        for (int i = 0; i < KF; i++) {
+            kf[i] = load_k(0, i, k_at);
+            if (i >= 2 * AHEAD - 1) {  // (all of them for heads of up to 128)
+                score(0, i - (2 * AHEAD - 1), kf[i - (2 * AHEAD - 1)]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            f16x8 vf[2][2];
+        }
 #pragma unroll
-            for (int q = 0; q < 2; q++) vf[0][q] = load_v(0, 0, q, v_at);
-            refer(1, [&] {
-                values(0, v_at);
+        for (int i = KF < 2 * AHEAD ? 0 : KF - (2 * AHEAD - 1); i < KF; i++) score(0, i, kf[i]);
+        fetch(1 - buf);
+        look(u + 2);
 #pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    ph[0][q] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-                    if constexpr (NQ == 2) pl[0][q] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-                }
-            });
-            sub = shift();
+        for (int i = 0; i < AHEAD; i++) kf[i] = load_k(1, i, k_at);
+        if (partial) {
+            clear(key0, buf);
+            hide(0, key0);
+        }
+        refer(0, [&](float alpha) { l *= alpha; });
+        float sub = shift();
+        const float before = l;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < KF; i++) {
+            if (i + AHEAD < KF) kf[i + AHEAD] = load_k(1, i + AHEAD, k_at);
+            score(1, i, kf[i]);
+#pragma unroll
+            for (int j = i * 16 / KF; j < (i + 1) * 16 / KF; j++) weight(0, j, sub);
             __builtin_amdgcn_sched_barrier(0);
+        }
+        f16x8 vf[2][2];
 #pragma unroll
-            for (int k = 0; k < 2 * HB; k++) {  // block 0's values, then block 1's
+        for (int q = 0; q < 2; q++) vf[0][q] = load_v(0, 0, q, v_at);
+        if (partial) hide(1, key0);
+        refer(1, [&](float alpha) {
+            l = before * alpha;
+            sub = shift();
+#pragma unroll
+            for (int j = 0; j < 16; j++) weight(0, j, sub);
+        });
+        sub = shift();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2 * HB; k++) {  // block 0's values, then block 1's
                 const int hb = k % HB, b = k / HB, nhb = (k + 1) % HB, nb = (k + 1) / HB;
                 if (k + 1 < 2 * HB) {
 #pragma unroll
@@ -977,13 +1014,6 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-        } else {
-            refer(0, [] {});
-            const float sub = shift();
-#pragma unroll
-            for (int j = 0; j < 16; j++) weight(0, j, sub);
-            values(0, v_at);
-        }
         lds_arrived();
     };
     // Any unit: rows that do not see all of it have scores of -inf.  Keys that no row sees are cleared in V, so that what
@@ -992,35 +1022,14 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         fetch(1 - buf);
         look(u + 2);
         const int32_t key0 = (int32_t)(u * BN);
-        if (key0 < sp.lo || is_partial(key0)) {
-#pragma unroll 1
-            for (int i = 0; i < NCH; i++) {
-                const uint32_t p = i * 256 + tid;
-                const int32_t key = key0 + (int32_t)(p / CPR);
-                __attribute__((address_space(3))) u32x4* at = (__attribute__((address_space(3))) u32x4*)(lds + (2 + buf) * BUF + p * 16);
-                if (key < sp.lo || key >= sp.hi) {
-                    *at = u32x4{0u, 0u, 0u, 0u};
-                } else {
-                    const u32x4 t = *at;
-                    if (att_nonfinite(t)) {
-                        odd = true;
-                        *at = att_clear_nonfinite(t);
-                    }
-                }
-            }
-            __syncthreads();
-        }
+        if (key0 < sp.lo || is_partial(key0)) clear(key0, buf);
         if (wave_on && key0 <= wpos1 && (!a.window || key0 + BN - 1 > wpos0 - (int32_t)a.window)) {
 #pragma unroll
             for (int b = 0; b < KB; b++) {
 #pragma unroll
                 for (int i = 0; i < KF; i++) score(b, i, load_k(b, i, buf * BUF));
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int32_t key = key0 + b * 32 + 8 * (j >> 2) + 4 * (int32_t)hf + (j & 3);
-                    if (key > pos || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
-                }
-                refer(b, [] {});
+                hide(b, key0);
+                refer(b, [&](float alpha) { l *= alpha; });
                 const float sub = shift();
 #pragma unroll
                 for (int j = 0; j < 16; j++) weight(b, j, sub);
@@ -1034,7 +1043,8 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     uint32_t f0 = max(sp.u0, (uint32_t)max(0, (max(w0, sp.lo) + BN - 1) / BN)), f1 = min(sp.u1, (uint32_t)max(0, w1 / BN));
     f0 = min(f0, sp.u1);
     f1 = f1 > f0 && wave_on ? f0 + ((f1 - f0) & ~1u) : f0;
-    const uint32_t parity = f0 & 1;
+    constexpr bool ONE = HD == 256;  // two such bodies do not fit the registers: one for all units, in pairs from the first
+    const uint32_t parity = ONE ? sp.u0 & 1 : f0 & 1;
     if (sp.u0 < sp.u1) {
         look(sp.u0);
         fetch((sp.u0 ^ parity) & 1);
@@ -1042,16 +1052,24 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     }
     lds_arrived();
     uint32_t u = sp.u0, stop = f0;
+    if constexpr (ONE) {
 #pragma unroll 1
-    for (;;) {
-#pragma unroll 1
-        for (; u < stop; u++) part_seen(u, (u ^ parity) & 1);
-        if (u >= sp.u1) break;
-        for (; u < f1; u += 2) {
-            whole(u, std::integral_constant<uint32_t, 0>());
-            whole(u + 1, std::integral_constant<uint32_t, 1>());
+        for (; u < sp.u1; u += 2) {  // (behind the last unit: keys that no row sees)
+            whole(u, std::integral_constant<uint32_t, 0>(), std::true_type());
+            whole(u + 1, std::integral_constant<uint32_t, 1>(), std::true_type());
         }
-        stop = sp.u1;
+    } else {
+#pragma unroll 1
+        for (;;) {
+#pragma unroll 1
+            for (; u < stop; u++) part_seen(u, (u ^ parity) & 1);
+            if (u >= sp.u1) break;
+            for (; u < f1; u += 2) {
+                whole(u, std::integral_constant<uint32_t, 0>(), std::false_type());
+                whole(u + 1, std::integral_constant<uint32_t, 1>(), std::false_type());
+            }
+            stop = sp.u1;
+        }
     }
     att_report(a, bad);
     if (tid == 0) *(__attribute__((address_space(3))) uint32_t*)lds = 0;
@@ -1111,10 +1129,10 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     }
 ATTEND_CHUNK(f16_t, f16, 64, 64, 2)
 ATTEND_CHUNK(f16_t, f16, 128, 64, 2)
-ATTEND_CHUNK(f16_t, f16, 256, 32, 1)
+ATTEND_CHUNK(f16_t, f16, 256, 64, 1)
 ATTEND_CHUNK(float, f32, 64, 64, 2)
 ATTEND_CHUNK(float, f32, 128, 64, 1)
-ATTEND_CHUNK(float, f32, 256, 32, 1)
+ATTEND_CHUNK(float, f32, 256, 64, 1)
 
 // ------------------------------------------------------------------------------------------- joining the parts
 // The tiles that were cut: a workgroup of eight waves takes join_rows rows of one listed tile and kv head.  Of up
