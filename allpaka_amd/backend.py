@@ -627,11 +627,35 @@ class PageStep:
     """What one PagedCache.extend hands out: the rows of every sequence (q_off), their positions and cache rows (slots)."""
 
     def __init__(self, n_seq, rows, device):
-        def buf(*shape):
-            return torch.empty(shape, dtype=torch.int32, device=device)
+        self.n_seq, self.rows = n_seq, rows
+        # one buffer: q_off [n_seq + 1], positions [rows], slots [rows], the pairs [n_seq, 2] copied and their number
+        self._buf = torch.empty(n_seq + 1 + 2 * rows + 2 * n_seq + 1, dtype=torch.int32, device=device)
+        at = self._buf.data_ptr()
+        sizes = (n_seq + 1, rows, rows, 2 * n_seq, 1)
+        self._ptrs = [at + 4 * sum(sizes[:i]) for i in range(5)]
 
-        self.q_off, self.positions, self.slots = buf(n_seq + 1), buf(rows), buf(rows)
-        self.pairs, self.n_pairs = buf(max(n_seq, 1), 2), buf(1)
+    @property
+    def q_off(self):
+        return self._buf[:self.n_seq + 1]
+
+    @property
+    def positions(self):
+        return self._buf[self.n_seq + 1:self.n_seq + 1 + self.rows]
+
+    @property
+    def slots(self):
+        return self._buf[self.n_seq + 1 + self.rows:self.n_seq + 1 + 2 * self.rows]
+
+    @property
+    def pairs(self):
+        """(to, from) of the pages that were copied, the first n_pairs of them."""
+        at = self.n_seq + 1 + 2 * self.rows
+        return self._buf[at:at + 2 * self.n_seq].view(self.n_seq, 2)
+
+    @property
+    def n_pairs(self):
+        """The number of pages that were copied."""
+        return self._buf[-1:]
 
 
 class PagedCache:
@@ -645,19 +669,23 @@ class PagedCache:
         self.b, self.region, self.page_size = backend, region, page_size
         self.n_pages, self.n_seq, self.max_pages = region.shape[1] // page_size, n_seq, max_pages
         dev = backend.device
-        self.pool = torch.zeros(backend.L.apk_pages_words(self.n_pages), dtype=torch.int32, device=dev)
-        self.page_table = torch.full((n_seq, max_pages), -1, dtype=torch.int32, device=dev)
-        self.kv_len = torch.zeros(n_seq, dtype=torch.int32, device=dev)
+        words = backend.L.apk_pages_words(self.n_pages)
+        # one buffer, so that its state is saved and restored by one copy
+        self._all = torch.zeros(words + n_seq * max_pages + n_seq, dtype=torch.int32, device=dev)
+        self.pool = self._all[:words]
+        self.page_table = self._all[words:words + n_seq * max_pages].view(n_seq, max_pages)
+        self.kv_len = self._all[words + n_seq * max_pages:]
+        self.page_table.fill_(-1)
         self._moves = torch.empty((max(self.n_pages // 2, 1), 2), dtype=torch.int32, device=dev)
         self._n_moves = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._state = (backend.h, _ptr(self.pool), self.n_pages, page_size, _ptr(self.page_table), max_pages, _ptr(self.kv_len), n_seq)
+        planes, capacity, width = region.shape
+        self._planes = (backend.h, _ptr(region), planes, capacity * width * 2, self.n_pages, page_size * width * 2)
         self._recount()
-
-    def _state(self):
-        return (self.b.h, _ptr(self.pool), self.n_pages, self.page_size, _ptr(self.page_table), self.max_pages, _ptr(self.kv_len), self.n_seq)
 
     def _recount(self):
         self.b._order()
-        check(self.b.L.apk_pages_init(*self._state()))
+        check(self.b.L.apk_pages_init(*self._state))
 
     @property
     def refs(self):
@@ -670,21 +698,28 @@ class PagedCache:
         self.b.sync()
         return int(self.pool[0].item())
 
+    def _torch_next(self):
+        """Before torch itself works on the state: what this context has queued comes first."""
+        assert not self.b._recording, "only what the context enqueues is recorded"
+        if torch.cuda.current_stream(self.b.device).cuda_stream != 0:
+            self.b.sync()
+
     def adopt(self, page_table, kv_len):
         """Takes over tables filled elsewhere; the pool is counted afresh."""
         assert page_table.shape == self.page_table.shape and kv_len.shape == self.kv_len.shape
+        self._torch_next()
         self.page_table.copy_(page_table)
         self.kv_len.copy_(kv_len)
         self._recount()
 
     def save(self):
-        """The state (not the cache rows) as copies, for restore."""
+        """The state (not the cache rows) as a copy, for restore."""
         self.b.sync()
-        return self.pool.clone(), self.page_table.clone(), self.kv_len.clone()
+        return self._all.clone()
 
     def restore(self, saved):
-        for t, s in zip((self.pool, self.page_table, self.kv_len), saved):
-            t.copy_(s)
+        self._torch_next()
+        self._all.copy_(saved)
 
     def _ids(self, t, n=None):
         assert t.dtype == torch.int32 and t.device == self.b.device and (n is None or t.numel() == n)
@@ -694,34 +729,32 @@ class PagedCache:
         """n_new int32 [n_seq] more tokens; rows: the most there can be in all.  Shared pages that get written to are copied
         in every plane.  Returns the PageStep (step: one to fill, of this n_seq and rows)."""
         step = PageStep(self.n_seq, rows, self.b.device) if step is None else step
-        assert step.positions.numel() == rows and step.q_off.numel() == self.n_seq + 1
+        assert step.rows == rows and step.n_seq == self.n_seq
         self.b._order()
-        check(self.b.L.apk_pages_extend(*self._state(), self._ids(n_new, self.n_seq), rows, _ptr(step.q_off), _ptr(step.positions),
-                                        _ptr(step.slots), _ptr(step.pairs), _ptr(step.n_pairs)))
-        self._copy(step.pairs, step.n_pairs, self.n_seq)
+        q_off, positions, slots, pairs, n_pairs = step._ptrs
+        check(self.b.L.apk_pages_extend(*self._state, self._ids(n_new, self.n_seq), rows, q_off, positions, slots, pairs, n_pairs))
+        self._copy(pairs, n_pairs, self.n_seq)
         return step
 
     def fork(self, src, dst):
         """Sequences dst (holding nothing) become further holders of the pages of sequences src."""
         assert src.numel() == dst.numel()
         self.b._order()
-        check(self.b.L.apk_pages_fork(*self._state(), self._ids(src), self._ids(dst), src.numel()))
+        check(self.b.L.apk_pages_fork(*self._state, self._ids(src), self._ids(dst), src.numel()))
 
     def truncate(self, new_len):
         """Cuts sequences to new_len int32 [n_seq] tokens; -1 leaves one as it is, 0 frees it."""
         self.b._order()
-        check(self.b.L.apk_pages_truncate(*self._state(), self._ids(new_len, self.n_seq)))
+        check(self.b.L.apk_pages_truncate(*self._state, self._ids(new_len, self.n_seq)))
 
     def compact(self):
         """Moves the pages in use to the front of every plane."""
         self.b._order()
-        check(self.b.L.apk_pages_compact(*self._state(), _ptr(self._moves), _ptr(self._n_moves)))
-        self._copy(self._moves, self._n_moves, max(self.n_pages // 2, 1))
+        check(self.b.L.apk_pages_compact(*self._state, _ptr(self._moves), _ptr(self._n_moves)))
+        self._copy(_ptr(self._moves), _ptr(self._n_moves), max(self.n_pages // 2, 1))
 
     def _copy(self, pairs, n_pairs, most):
-        planes, capacity, width = self.region.shape
-        check(self.b.L.apk_pages_copy(self.b.h, _ptr(self.region), planes, capacity * width * 2, self.n_pages, self.page_size * width * 2,
-                                      _ptr(pairs), _ptr(n_pairs), most))
+        check(self.b.L.apk_pages_copy(*self._planes, pairs, n_pairs, most))
 
 
 class _Recording:

@@ -1839,10 +1839,12 @@ int apk_pages_copy(apk_ctx* c, void* region, size_t n_planes, size_t plane_bytes
     if (int rc = set_device(c)) return rc;
     uint32_t np = (uint32_t)n_pages, npl = (uint32_t)n_planes, mp = (uint32_t)max_pairs;
     uint64_t plb = plane_bytes, pgb = page_bytes;
-    uint32_t slices = (uint32_t)((page_bytes / 16 + 1023) / 1024);
+    const uint64_t tiles = page_bytes / 16;
+    uint32_t slices = (uint32_t)((tiles + 1023) / 1024), span = (uint32_t)((tiles + slices - 1) / slices);
+    if (max_pairs > 0xffffffffu / slices) return fail(APK_DECLINE_SHAPE, "apk_pages_copy: too large");
     const double items = (double)max_pairs * (double)n_planes * slices;
-    const unsigned grid = items < 4096. ? (unsigned)items : 4096u;
-    void* args[] = {&region, &npl, &plb, &np, &pgb, &pairs, &n_pairs, &mp, &slices, &c->fault_dev};
+    const unsigned grid = items < 8192. ? (unsigned)items : 8192u;
+    void* args[] = {&region, &npl, &plb, &np, &pgb, &pairs, &n_pairs, &mp, &slices, &span, &c->fault_dev};
     return launch(c, "apk_pages_copy_k", grid, 256, 0, args);
 }
 

@@ -33,6 +33,7 @@ DEV void pg_sync() {  // everything the workgroup has written is in the L2 befor
     __syncthreads();
 }
 #define PG_BLOCK 1024
+#define PG_LIST 4096  // new pages of a step that fit LDS
 // Inclusive sums over the workgroup of up to 1024 lanes; `total`: of all.  sm: 17 words.
 DEV uint32_t pg_scan(uint32_t v, uint32_t* sm, uint32_t& total) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -53,6 +54,46 @@ DEV uint32_t pg_scan(uint32_t v, uint32_t* sm, uint32_t& total) {
         total += t;
     }
     return v + before;
+}
+// The same for three values at once; v0 .. v2 become their sums up to this lane.  sm: 48 words.
+DEV void pg_scan3(uint32_t& v0, uint32_t& v1, uint32_t& v2, uint32_t* sm, uint32_t& t0, uint32_t& t1, uint32_t& t2) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t a = __shfl_up(v0, d), b = __shfl_up(v1, d), c = __shfl_up(v2, d);
+        if ((int)lane >= d) {
+            v0 += a;
+            v1 += b;
+            v2 += c;
+        }
+    }
+    __syncthreads();
+    if (lane == 63) {
+        sm[wave] = v0;
+        sm[16 + wave] = v1;
+        sm[32 + wave] = v2;
+    }
+    __syncthreads();
+    uint32_t b0 = 0, b1 = 0, b2 = 0;
+    t0 = t1 = t2 = 0;
+#pragma unroll
+    for (int w = 0; w < PG_BLOCK / 64; w++) {
+        const bool before = (uint32_t)w < wave;
+        b0 += before ? sm[w] : 0;
+        b1 += before ? sm[16 + w] : 0;
+        b2 += before ? sm[32 + w] : 0;
+        t0 += sm[w];
+        t1 += sm[16 + w];
+        t2 += sm[32 + w];
+    }
+    v0 += b0;
+    v1 += b1;
+    v2 += b2;
+}
+DEV uint64_t pg_wave_sum(uint64_t v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
 }
 // The last index i of off[0 .. n) (ascending, off[0] <= k) with off[i] <= k.
 DEV uint32_t pg_find(const uint32_t* off, uint32_t n, uint32_t k) {
@@ -79,13 +120,13 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_init_k(uint32_t
         pg_st(P.last + i, 0);
     }
     pg_sync();
-    for (uint32_t s = 0; s < n_seq; s++) {
+    for (uint32_t s = tid >> 6; s < n_seq; s += PG_BLOCK / 64) {  // a wave per sequence
         uint32_t used = pg_ceil(kv_len[s], page);
         if (used > max_pages) {
             used = max_pages;
-            if (tid == 0) atomicOr(fault, APK_FAULT_CACHE_RANGE);
+            if ((tid & 63) == 0) atomicOr(fault, APK_FAULT_CACHE_RANGE);
         }
-        for (uint32_t j = tid; j < used; j += PG_BLOCK) {
+        for (uint32_t j = tid & 63; j < used; j += 64) {
             const uint32_t e = table[(uint64_t)s * max_pages + j];
             if (e < n_pages) pg_add(P.refs + e, 1);
             else atomicOr(fault, APK_FAULT_CACHE_RANGE);
@@ -113,13 +154,18 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_extend_k(uint32
     const page_pool P = page_pool::at(pool, n_pages);
     const uint32_t tid = threadIdx.x;
     const uint64_t cap = (uint64_t)max_pages * page;
-    __shared__ uint32_t sm[PG_BLOCK / 64 + 1], bad;
+    __shared__ uint32_t sm[3 * PG_BLOCK / 64], bad, shared_tails;
     __shared__ unsigned long long sum_new, sum_need;
-    __shared__ uint32_t row_off[PG_BLOCK + 1], first[PG_BLOCK + 1], s_len[PG_BLOCK], s_have[PG_BLOCK];
+    __shared__ uint32_t row_off[PG_BLOCK + 1], first[PG_BLOCK + 1], s_len[PG_BLOCK], s_have[PG_BLOCK], s_tail[PG_BLOCK];
+    __shared__ uint32_t s_list[PG_LIST];
     if (tid == 0) {
-        bad = 0;
+        bad = shared_tails = 0;
         sum_new = sum_need = 0;
     }
+    // What does not depend on the sequences is asked for first: the number of free pages and this lane's first word of them.
+    const uint32_t per = (P.words + PG_BLOCK - 1) / PG_BLOCK;
+    const uint32_t w0 = min(tid * per, P.words), w1 = min(w0 + per, P.words);
+    const uint32_t free0 = pg_ld(P.head), word0 = pg_ld(P.bits + min(w0, P.words - 1));
     // the page that a sequence's next token falls into, where it holds one already; n_pages: none
     auto tail_of = [&](uint32_t s, uint32_t len, uint32_t fresh) -> uint32_t {
         if (!fresh || len % page == 0 || len > cap) return n_pages;
@@ -129,33 +175,70 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_extend_k(uint32
         return n_pages;
     };
     __syncthreads();
+    // (the first block of sequences keeps what it reads)
+    uint32_t len_a = 0, new_a = 0, tail_a = n_pages, held_a = 0;
+    auto sequence = [&](uint32_t s, uint32_t& len, uint32_t& fresh, uint32_t& t, uint32_t& held) {
+        if (s == tid) {
+            len = len_a;
+            fresh = new_a;
+            t = tail_a;
+            held = held_a;
+        } else {
+            len = kv_len[s];
+            fresh = n_new[s];
+            t = tail_of(s, len, fresh);
+            held = t < n_pages ? pg_ld(P.refs + t) : 0;
+        }
+    };
+    if (tid < n_seq) {
+        len_a = kv_len[tid];
+        new_a = n_new[tid];
+        tail_a = tail_of(tid, len_a, new_a);
+        held_a = tail_a < n_pages ? pg_ld(P.refs + tail_a) : 0;
+    }
     // who writes into a page that others hold: their number and the last of them
     for (uint32_t s = tid; s < n_seq; s += PG_BLOCK) {
-        const uint32_t len = kv_len[s], fresh = n_new[s], t = tail_of(s, len, fresh);
-        if (t < n_pages && pg_ld(P.refs + t) > 1) {
+        uint32_t len, fresh, t, held;
+        sequence(s, len, fresh, t, held);
+        if (held > 1) {
             pg_add(P.cnt + t, 1);
             __hip_atomic_fetch_max(P.last + t, s + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            shared_tails = 1;
         }
         if ((uint64_t)len + fresh > cap) bad = APK_FAULT_CACHE_RANGE;
     }
-    pg_sync();
+    __syncthreads();
+    if (shared_tails) pg_sync();
     // of the holders of a page that all write now the last one keeps it, the others write to a copy
-    auto copies = [&](uint32_t s, uint32_t t) -> uint32_t {
-        if (t >= n_pages) return 0;
-        const uint32_t held = pg_ld(P.refs + t);
+    auto copies = [&](uint32_t s, uint32_t t, uint32_t held) -> uint32_t {
         return held > 1 && !(pg_ld(P.cnt + t) == held && pg_ld(P.last + t) == s + 1);
     };
-    for (uint32_t s = tid; s < n_seq; s += PG_BLOCK) {
-        const uint32_t len = kv_len[s], fresh = n_new[s];
-        if ((uint64_t)len + fresh > cap) continue;
-        const uint32_t need = pg_ceil(len + fresh, page) - pg_ceil(len, page) + copies(s, tail_of(s, len, fresh));
-        atomicAdd(&sum_new, (unsigned long long)fresh);
-        atomicAdd(&sum_need, (unsigned long long)need);
+    uint32_t need_a = 0, copy_a = 0;
+    {
+        uint64_t my_new = 0, my_need = 0;
+        for (uint32_t s = tid; s < n_seq; s += PG_BLOCK) {
+            uint32_t len, fresh, t, held;
+            sequence(s, len, fresh, t, held);
+            if ((uint64_t)len + fresh > cap) continue;
+            const uint32_t cp = copies(s, t, held), need = pg_ceil(len + fresh, page) - pg_ceil(len, page) + cp;
+            my_new += fresh;
+            my_need += need;
+            if (s == tid) {
+                need_a = need;
+                copy_a = cp;
+            }
+        }
+        my_new = pg_wave_sum(my_new);
+        my_need = pg_wave_sum(my_need);
+        if ((tid & 63) == 0) {
+            if (my_new) atomicAdd(&sum_new, (unsigned long long)my_new);
+            if (my_need) atomicAdd(&sum_need, (unsigned long long)my_need);
+        }
     }
-    pg_sync();
-    const uint32_t free0 = pg_ld(P.head);
+    __syncthreads();
     const bool full = sum_need > min(free0, n_pages), many = sum_new > rows;
     if (bad || full || many) {  // nothing is changed but the scratch put back
+        pg_sync();
         for (uint32_t s = tid; s < n_seq; s += PG_BLOCK) {
             const uint32_t t = tail_of(s, kv_len[s], n_new[s]);
             if (t < n_pages) {
@@ -175,63 +258,69 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_extend_k(uint32
         }
         return;
     }
-    // the lowest sum_need free pages, ascending
+    // the lowest sum_need free pages, ascending; a short list stays in LDS
     const uint32_t total_need = (uint32_t)sum_need;
+    auto fresh_page = [&](uint32_t k) { return total_need <= PG_LIST ? s_list[min(k, (uint32_t)PG_LIST - 1)] : pg_ld(P.list + k); };
     if (total_need) {
-        const uint32_t per = (P.words + PG_BLOCK - 1) / PG_BLOCK;
-        const uint32_t w0 = min(tid * per, P.words), w1 = min(w0 + per, P.words);
+        auto word = [&](uint32_t w) {
+            return (w == w0 ? word0 : pg_ld(P.bits + w)) & (w * 32 + 32 > n_pages ? (1u << (n_pages & 31)) - 1 : 0xffffffffu);
+        };
         uint32_t mine = 0, all;
-        for (uint32_t w = w0; w < w1; w++) mine += (uint32_t)__popc(pg_ld(P.bits + w));
+        for (uint32_t w = w0; w < w1; w++) mine += (uint32_t)__popc(word(w));
         uint32_t k = pg_scan(mine, sm, all) - mine;
         for (uint32_t w = w0; w < w1 && k < total_need; w++) {
-            uint32_t b = pg_ld(P.bits + w) & (w * 32 + 32 > n_pages ? (1u << (n_pages & 31)) - 1 : 0xffffffffu);
+            uint32_t b = word(w);
             while (b && k < total_need) {
                 const uint32_t p = w * 32 + (uint32_t)__builtin_ctz(b);
                 b &= b - 1;
-                pg_st(P.list + k++, p);
+                if (total_need <= PG_LIST) s_list[k] = p;
+                else pg_st(P.list + k, p);
+                k++;
                 pg_st(P.refs + p, 1);
             }
             pg_st(P.bits + w, b);
         }
         if (tid == 0) pg_st(P.head, free0 - total_need);
+        if (total_need > PG_LIST) pg_sync();  // (a short list: seen behind the next barrier)
     }
-    pg_sync();
     uint32_t row_base = 0, need_base = 0, pair_base = 0;
     for (uint32_t base = 0; base < n_seq; base += PG_BLOCK) {
         const uint32_t s = base + tid, here = min((uint32_t)PG_BLOCK, n_seq - base);
-        uint32_t len = 0, fresh = 0, need = 0, cp = 0, have = 0, t = n_pages;
+        uint32_t len = 0, fresh = 0, need = 0, cp = 0, have = 0, t = n_pages, held = 0;
         if (s < n_seq) {
-            len = kv_len[s];
-            fresh = n_new[s];
+            sequence(s, len, fresh, t, held);
             have = pg_ceil(len, page);
-            t = tail_of(s, len, fresh);
-            cp = copies(s, t);
-            need = pg_ceil(len + fresh, page) - have + cp;
+            if (base == 0) {
+                cp = copy_a;
+                need = need_a;
+            } else {
+                cp = copies(s, t, held);
+                need = pg_ceil(len + fresh, page) - have + cp;
+            }
         }
-        uint32_t all_new, all_need, all_cp;
-        const uint32_t i_new = pg_scan(fresh, sm, all_new), i_need = pg_scan(need, sm, all_need), i_cp = pg_scan(cp, sm, all_cp);
+        uint32_t i_new = fresh, i_need = need, i_cp = cp, all_new, all_need, all_cp;
+        pg_scan3(i_new, i_need, i_cp, sm, all_new, all_need, all_cp);
         if (tid < here) {
             row_off[tid] = i_new - fresh;
             first[tid] = i_need - need;
             s_len[tid] = len;
             s_have[tid] = have - cp;  // item first + k goes to table entry have + k; a copy's replaces the entry before
+            s_tail[tid] = t;
             q_off[s + 1] = row_base + i_new;
         }
-        pg_sync();
-        // (every decision of this block is made: references may change now; later blocks of sequences decide by cnt and
-        // refs of pages they share with this one, so references to those drop only at the very end)
+        __syncthreads();
+        // (references of pages that others hold drop only at the very end: later blocks of sequences decide by them)
         if (cp) {
-            pairs[2 * (pair_base + i_cp - 1)] = pg_ld(P.list + need_base + i_need - need);
+            pairs[2 * (pair_base + i_cp - 1)] = fresh_page(need_base + i_need - need);
             pairs[2 * (pair_base + i_cp - 1) + 1] = t;
         }
         for (uint32_t k = tid; k < all_need; k += PG_BLOCK) {
             const uint32_t i = pg_find(first, here, k);
-            pg_st(table + (uint64_t)(base + i) * max_pages + s_have[i] + (k - first[i]), pg_ld(P.list + need_base + k));
+            pg_st(table + (uint64_t)(base + i) * max_pages + s_have[i] + (k - first[i]), fresh_page(need_base + k));
         }
-        pg_sync();
         for (uint32_t r = tid; r < all_new; r += PG_BLOCK) {
-            const uint32_t i = pg_find(row_off, here, r), pos = s_len[i] + (r - row_off[i]);
-            const uint32_t e = pg_ld(table + (uint64_t)(base + i) * max_pages + pos / page);
+            const uint32_t i = pg_find(row_off, here, r), pos = s_len[i] + (r - row_off[i]), j = pos / page;
+            const uint32_t e = j >= s_have[i] ? fresh_page(need_base + first[i] + (j - s_have[i])) : s_tail[i];
             positions[row_base + r] = pos;
             slots[row_base + r] = e * page + pos % page;
         }
@@ -239,13 +328,16 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_extend_k(uint32
         row_base += all_new;
         need_base += all_need;
         pair_base += all_cp;
-        pg_sync();
+        if (base + PG_BLOCK < n_seq) pg_sync();
     }
-    for (uint32_t i = tid; i < pair_base; i += PG_BLOCK) {
-        const uint32_t t = pg_ld(pairs + 2 * i + 1);
-        pg_add(P.refs + t, 0xffffffffu);
-        pg_st(P.cnt + t, 0);
-        pg_st(P.last + t, 0);
+    if (pair_base) {
+        pg_sync();
+        for (uint32_t i = tid; i < pair_base; i += PG_BLOCK) {
+            const uint32_t t = pg_ld(pairs + 2 * i + 1);
+            pg_add(P.refs + t, 0xffffffffu);
+            pg_st(P.cnt + t, 0);
+            pg_st(P.last + t, 0);
+        }
     }
     for (uint32_t r = row_base + tid; r < rows; r += PG_BLOCK) {  // rows of nobody: no cache row, so that a store skips them
         positions[r] = 0;
@@ -429,32 +521,42 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_compact_k(uint3
     if (tid == 0) *n_pairs = moves;
 }
 
-// Page pairs[2 i + 1] copied over page pairs[2 i] in every plane, *n_pairs of them (at most max_pairs).  A workgroup takes
-// slices of 256 lanes x 4 tiles of 16 bytes in turn.  Bound by memory: a plain copy whose addresses come out of a list.
+// Page pairs[2 i + 1] copied over page pairs[2 i] in every plane, *n_pairs of them (at most max_pairs).  An item is one slice
+// (span tiles of 16 bytes, no more than 4 per lane) of one pair in one plane; workgroups take items in turn, plane after
+// plane.  Bound by memory: a plain copy whose addresses come out of a list.  1.2 GB in pages of 32 KiB move in 235 us
+// (5.3 TB/s, a copy of one piece 6.7).  The reads stay in the caches: 32 copies of one shared page in 64 planes take 33 us,
+// 60 with reads marked as not to be kept, which move distinct pages in 230; planes side by side instead of one after the
+// other take 250.
 extern "C" __global__ __launch_bounds__(256) void apk_pages_copy_k(char* region, uint32_t n_planes, uint64_t plane_bytes, uint32_t n_pages,
                                                                    uint64_t page_bytes, const uint32_t* pairs, const uint32_t* n_pairs,
-                                                                   uint32_t max_pairs, uint32_t slices, uint32_t* fault) {
-    const uint32_t n = min(*n_pairs, max_pairs);
+                                                                   uint32_t max_pairs, uint32_t slices, uint32_t span, uint32_t* fault) {
+    const uint32_t n = min(*n_pairs, max_pairs), per = n * slices;  // items of a plane
+    if (per == 0) return;
     const uint32_t tiles = (uint32_t)(page_bytes / 16);
-    const uint64_t items = (uint64_t)n * n_planes * slices;
-    for (uint64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const uint32_t slice = (uint32_t)(it % slices);
-        const uint64_t rest = it / slices;
-        const uint32_t i = (uint32_t)(rest % n), plane = (uint32_t)(rest / n);
-        const uint32_t to = pairs[2 * i], from = pairs[2 * i + 1];
+    uint32_t plane = blockIdx.x / per, r = blockIdx.x % per;
+    const uint32_t dp = gridDim.x / per, dr = gridDim.x % per;
+    while (plane < n_planes) {
+        const uint32_t i = r / slices, t0 = (r % slices) * span + threadIdx.x, t1 = min((r % slices + 1) * span, tiles);
+        const uint32_t to = pairs[2 * (uint64_t)i], from = pairs[2 * (uint64_t)i + 1];
+        char* const base = region + plane * plane_bytes;
+        r += dr;
+        plane += dp;
+        if (r >= per) {
+            r -= per;
+            plane++;
+        }
         if (to >= n_pages || from >= n_pages) {
             if (threadIdx.x == 0) atomicOr(fault, APK_FAULT_CACHE_RANGE);
             continue;
         }
-        char* base = region + plane * plane_bytes;
         const u32x4* src = (const u32x4*)(base + from * page_bytes);
         char* dst = base + to * page_bytes;
-        const uint32_t t0 = slice * 1024 + threadIdx.x;
         u32x4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = __builtin_nontemporal_load(src + (t0 + k * 256 < tiles ? t0 + k * 256 : 0));
+        for (int k = 0; k < 4; k++)
+            v[k] = src[t0 + k * 256 < t1 ? t0 + k * 256 : 0];
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (t0 + k * 256 < tiles) nt_store(v[k], dst + (uint64_t)(t0 + k * 256) * 16);
+            if (t0 + k * 256 < t1) nt_store(v[k], dst + (uint64_t)(t0 + k * 256) * 16);
     }
 }
