@@ -670,11 +670,12 @@ class PagedCache:
         self.n_pages, self.n_seq, self.max_pages = region.shape[1] // page_size, n_seq, max_pages
         dev = backend.device
         words = backend.L.apk_pages_words(self.n_pages)
-        # one buffer, so that its state is saved and restored by one copy
-        self._all = torch.zeros(words + n_seq * max_pages + n_seq, dtype=torch.int32, device=dev)
+        # one buffer of whole 16-byte tiles, so that the state is saved and restored by one copy
+        total = words + n_seq * max_pages + n_seq
+        self._all = torch.zeros((total + 3) // 4 * 4, dtype=torch.int32, device=dev)
         self.pool = self._all[:words]
         self.page_table = self._all[words:words + n_seq * max_pages].view(n_seq, max_pages)
-        self.kv_len = self._all[words + n_seq * max_pages:]
+        self.kv_len = self._all[total - n_seq:total]
         self.page_table.fill_(-1)
         self._moves = torch.empty((max(self.n_pages // 2, 1), 2), dtype=torch.int32, device=dev)
         self._n_moves = torch.zeros(1, dtype=torch.int32, device=dev)
@@ -718,8 +719,10 @@ class PagedCache:
         return self._all.clone()
 
     def restore(self, saved):
-        self._torch_next()
-        self._all.copy_(saved)
+        """The state of a save again."""
+        assert saved.dtype == torch.int32 and saved.device == self.b.device and saved.numel() == self._all.numel()
+        self.b._order()
+        check(self.b.L.apk_copy(self.b.h, _ptr(saved), self._all.data_ptr(), 4 * self._all.numel()))
 
     def _ids(self, t, n=None):
         assert t.dtype == torch.int32 and t.device == self.b.device and (n is None or t.numel() == n)
