@@ -78,8 +78,7 @@ std::vector<std::string> all_kernel_names() {
                                   "apk_pages_init_k", "apk_pages_extend_k", "apk_pages_fork_k", "apk_pages_truncate_k", "apk_pages_compact_k", "apk_pages_copy_k"};
     for (const char* t : {"f32", "f16"}) {
         for (int hd : kAttendHeadDims) {
-            for (int nb : {1, 2, 4})
-                if (hd * nb <= 512) v.push_back(std::string("apk_attend_few_") + t + "_hd" + std::to_string(hd) + "_b" + std::to_string(nb));
+            v.push_back(std::string("apk_attend_few_") + t + "_hd" + std::to_string(hd));
             v.push_back(std::string("apk_attend_chunk_") + t + "_hd" + std::to_string(hd));
         }
         v.push_back(std::string("apk_attend_join_") + t);
@@ -1581,10 +1580,6 @@ int apk_argmax_rows(apk_ctx* c, const float* logits, size_t rows, size_t n, uint
 namespace {
 
 const size_t kAttendScratch = 256u << 20;
-#ifndef V_TT
-#define V_TT 256
-#define V_UM 2
-#endif
 
 // page / key arithmetic of the kernels: floor(2^32 / page), 2^32 - 1 for page 1
 uint32_t page_magic(size_t page) { return page == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / page); }
@@ -1639,62 +1634,58 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
         void* args[] = {&a};
         return launch(c, "apk_attend_any_" + t_name, (unsigned)(rows * n_q), 256, (unsigned)((5 * head_dim + 8) * 4), args);
     }
-    // Tiles of few rows (16, 32 or 64, whichever holds the rows of a sequence on average) read the cache straight into
-    // registers; more rows share it through LDS in tiles of 128.  (Heads of 256: 64 rows would not leave registers.)
+    // Tiles of 16 flat (token, head) rows read the cache straight into registers; tiles of 128 rows share it through LDS.
+    // The first form where the rows of a sequence are 16 at most on average (hd 128, f16, 16 sequences of 4000 keys, 8 kv
+    // heads, us of the small / the large tiles: 16 rows 66 / 65, 32 rows 81 / 74, 64 rows 149 / 74; f32 69 / 85, 83 / 87, 153 /
+    // 95; one sequence of 32000 keys, f16, 16 rows 38 / 77).
+    const uint64_t few_tiles = rows * (uint64_t)a.group / 16 + n_seq;
+    // Caches that are short whatever their lengths, in launches that do not fill the chip: a workgroup per tile of 16 rows
+    // and head, its waves sharing the keys; no joining launch.  (One sequence, 8 kv heads, us this way / cut into pieces: 600
+    // keys 14.2 / 16.6, 900 18.4 / 16.8, 1500 22.9 / 17.0; 8 sequences of 900 19.8 / 21.8; 8 drafts over 600 keys 16 / 22 with tiles of 128 rows.)
+    const uint64_t all_keys = max_pages * page_size;
+    const bool whole = all_keys <= 1024 && few_tiles * n_kv <= 256;
+    const bool few = whole || rows * (uint64_t)a.group <= 16 * (uint64_t)n_seq;
     unsigned shmem, block;
     std::string kernel;
-    const double flat = (double)rows * a.group / (double)n_seq;  // rows of a kv head per sequence
-    #ifndef V_NB1
-#define V_NB1 16.
-#define V_NB2 32.
-#endif
-    const unsigned nb = !q_off || flat <= V_NB1 ? 1 : flat <= V_NB2 ? 2 : flat <= 64. && head_dim < 256 ? 4 : 0;
-    if (nb) {
-        const unsigned waves = head_dim == 256 || (head_dim == 128 && nb == 4) ? 4 : 8;
-        a.tile_rows = 16 * nb;
+    if (few) {
+        const unsigned waves = head_dim == 256 ? 4 : 8;
+        a.tile_rows = 16;
         a.unit = 32;
         a.heads = 1;
-        while (a.heads < waves && n_kv % (2 * a.heads) == 0) a.heads *= 2;
-        a.unit_min = V_UM;
-        const unsigned r = !q_off && a.group < a.tile_rows ? a.group : a.tile_rows;
+        while (!whole && a.heads < waves && n_kv % (2 * a.heads) == 0) a.heads *= 2;
+        const unsigned r = !q_off && a.group < 16 ? a.group : 16;
         block = waves * 64;
-        shmem = a.heads == waves ? 0 : (unsigned)((2 * waves * a.tile_rows + waves * r * head_dim) * 4);
-        kernel = "apk_attend_few_" + t_name + "_hd" + std::to_string(head_dim) + "_b" + std::to_string(nb);
+        shmem = a.heads == waves ? 0 : (unsigned)((2 * waves * 16 + waves * r * head_dim) * 4);
+        kernel = "apk_attend_few_";
     } else {
         a.tile_rows = APK_ATT_CHUNK_ROWS;
         a.unit = 64;
         a.heads = 1;
-        a.target = 512;
-        a.unit_min = 512 / a.unit;
         block = 256;
         shmem = (unsigned)(4 * a.unit * head_dim * 2);
-        kernel = "apk_attend_chunk_" + t_name + "_hd" + std::to_string(head_dim);
+        kernel = "apk_attend_chunk_";
     }
+    kernel += t_name + "_hd" + std::to_string(head_dim);
     while ((1u << a.tile_shift) < a.tile_rows) a.tile_shift++;
     while ((1u << a.unit_shift) < a.unit) a.unit_shift++;
     const uint64_t tiles = rows * (uint64_t)a.group / a.tile_rows + n_seq;
     const uint64_t units = (max_pages * page_size + a.unit - 1) / a.unit;  // of a tile at most
     const size_t fit = (kAttendScratch - APK_ATT_PART_AT) / (2 * (size_t)a.tile_rows * (head_dim + 2) * 4);  // pairs of slots
+    const uint64_t hblocks = n_kv / a.heads;
     uint64_t items, listed;
     bool cut;
-    // Caches that are short whatever their lengths, in launches that do not fill the chip: a workgroup per tile and head,
-    // its waves sharing the keys.  (600 keys, 8 kv heads: one launch, no joining launch.)
-    const bool whole = nb && units <= 32 && tiles * n_kv <= 256;
     if (whole) {
-        const unsigned waves = block / 64;
-        a.heads = 1;
         a.unit_min = a.whole_units = (uint32_t)units;
-        shmem = (unsigned)((2 * waves * a.tile_rows + waves * a.tile_rows * head_dim) * 4);
-    }
-    const uint64_t hblocks = n_kv / a.heads;
-    if (whole) {
         a.target = (uint32_t)tiles;
         items = tiles;
         listed = 0;
         cut = false;
-    } else if (nb) {
-        // as many workgroups as fill the chip, each with at most two cut segments
-        uint64_t t = (V_TT + hblocks - 1) / hblocks;
+    } else if (few) {
+        // As many workgroups as there are CUs, each with a piece of all units, of two at least: at most two cut segments.
+        // (131071 keys, us with 128 / 256 / 512 workgroups: 122 / 108 / 119; 64 sequences of 6000: 325 / 277 / 297.  2000
+        // keys with pieces of 1 / 2 / 4 / 8 units at least: 16.1 / 17.7 / 20.6 / 28.6, 8000 keys 21.4 / 20.2 / 23.3 / 31.7.)
+        a.unit_min = 2;
+        uint64_t t = (256 + hblocks - 1) / hblocks;
         if (t * n_kv > fit) t = fit / n_kv;
         if (t > APK_ATT_MAX_LIST) t = APK_ATT_MAX_LIST;
         if (tiles * units < t * a.unit_min) t = (tiles * units + a.unit_min - 1) / a.unit_min;
@@ -1707,14 +1698,19 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
         cut = units > 1 && t > 1;
     } else {
         // A cut tile has at least two parts, of more than half of a part's share of all units: no more than 2 * target
-        // parts come of cutting, of no more than target tiles.
+        // parts come of cutting, of no more than target tiles.  Two workgroups a CU (us with 256 / 512 / 1024 for 512 tokens over
+        // 32000 keys: 729 / 677 / 694; heads of 256, one workgroup a CU: 311 / 304 / 420); parts of 256 / 512 / 1024 keys at
+        // least make no difference above 2 %.
+        a.target = 512;
+        a.unit_min = 512 / a.unit;
         if (a.target > fit) a.target = (uint32_t)fit;
         const uint64_t parts = units > a.unit_min ? (units + a.unit_min - 1) / a.unit_min : 1;
         items = tiles + (a.target + hblocks - 1) / hblocks + 1;
         if (tiles * parts < items) items = tiles * parts;
         listed = (a.target + hblocks - 1) / hblocks;
         if (tiles < listed) listed = tiles;
-        a.join_rows = 32;
+        // (few tiles are cut into many parts, whose rows one workgroup would join in turn)
+        for (a.join_rows = 32; a.join_rows > 1 && listed * n_kv * (a.tile_rows / a.join_rows) < 1024;) a.join_rows /= 2;
         cut = parts > 1;
     }
     if (items * hblocks > 0x7fffffffu) return fail(APK_DECLINE_SHAPE, "%s: too large", name);

@@ -379,17 +379,17 @@ DEV u32x4 att_clear_nonfinite(u32x4 t) {
     }
     return t;
 }
-// Single tokens, and chunks of a few: tiles of 16 NB flat rows.  A workgroup of W waves takes `heads` kv heads of one tile
+// Single tokens, and chunks of a few: tiles of 16 flat rows.  A workgroup of W waves takes `heads` kv heads of one tile
 // and part, W / heads waves to a head, each of them blocks of 32 keys in turn; so a workgroup reads whole rows of the
 // cache where there are W heads or more, and its waves need not be joined.  K and V go from memory straight to registers:
 // a wave's K block is the first operand of 16x16x32 products as it lies (16 bytes of a key a lane), its V block becomes
 // one by an in-lane transpose (8 keys x 8 channels a lane).  K of the next block is under way from the moment K of this
 // one is used up, V likewise.  Bound by the stream of K and V.
-template <typename T, int HD, int NB, int W>
+template <typename T, int HD, int W>
 DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     constexpr int KF = HD / 32;           // K fragments of 16 keys
     constexpr int CH = HD / 16;           // channels a lane holds of a V row
-    constexpr int NQ = att_q<T>::N, R = 16 * NB;
+    constexpr int NQ = att_q<T>::N, R = 16;
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
     const uint32_t hblocks = a.n_kv / a.heads, WK = W / a.heads;
     const uint32_t kvh = blockIdx.x % hblocks * a.heads + wave % a.heads, wk = wave / a.heads, piece = blockIdx.x / hblocks;
@@ -433,26 +433,17 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     const f16_t* kb = (const f16_t*)a.k + (uint64_t)kvh * HD;
     const f16_t* vb = (const f16_t*)a.v + (uint64_t)kvh * HD;
 
-    typename att_q<T>::raw_t qr[NB][KF];
-    float c[NB], m[NB], l[NB];
-    int32_t pos[NB];
-    uint64_t qat[NB];
+    typename att_q<T>::raw_t qr[KF];
+    const uint32_t flat = flat0 + n16, tok = flat / a.group;
+    const bool on = n16 < rows_here;
+    const uint64_t qat = on ? ((uint64_t)(it.s.row0 + tok) * a.n_q + kvh * a.group + flat % a.group) * HD : 0;
+    const int32_t pos = on ? it.s.p0 + (int32_t)tok : -1;
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        const uint32_t flat = flat0 + nb * 16 + n16, tok = flat / a.group;
-        const bool on = nb * 16 + n16 < rows_here;
-        qat[nb] = on ? ((uint64_t)(it.s.row0 + tok) * a.n_q + kvh * a.group + flat % a.group) * HD : 0;
-        pos[nb] = on ? it.s.p0 + (int32_t)tok : -1;
+    for (int s = 0; s < KF; s++) qr[s] = att_q<T>::load((const T*)a.q + qat + g * 8 + s * 32, on);
+    float m = NEG_INF, l = 0.f;
+    f32x4 o[CH];
 #pragma unroll
-        for (int s = 0; s < KF; s++) qr[nb][s] = att_q<T>::load((const T*)a.q + qat[nb] + g * 8 + s * 32, on);
-        m[nb] = NEG_INF;
-        l[nb] = 0.f;
-    }
-    f32x4 o[NB][CH];
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-        for (int i = 0; i < CH; i++) o[nb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < CH; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     typedef uint32_t vrow_t __attribute__((ext_vector_type(CH / 2)));
     const int32_t k_end = min((int32_t)(sp.u1 * 32), sp.hi), k_lo = max(sp.lo, (int32_t)(sp.u0 * 32));
@@ -495,33 +486,28 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
         load_v(row);
         __builtin_amdgcn_sched_barrier(0);
     }
-    f16x8 qf[NB][KF][NQ];
+    f16x8 qf[KF][NQ];
+    float mul = 1.f, inv = 1.f;
+    if constexpr (NQ == 2) {
+        float mx = 0.f;
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        float mul = 1.f, inv = 1.f;
-        if constexpr (NQ == 2) {
-            float mx = 0.f;
-#pragma unroll
-            for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qr[nb][s]));
-            att_q_scale(max_xor<32>(max_xor<16>(mx)), mul, inv);
-        }
-#pragma unroll
-        for (int s = 0; s < KF; s++) att_q<T>::split(qr[nb][s], mul * a.sign, qf[nb][s]);
-        c[nb] = a.c * inv;
+        for (int s = 0; s < KF; s++) mx = fmaxf(mx, att_q<T>::absmax(qr[s]));
+        att_q_scale(max_xor<32>(max_xor<16>(mx)), mul, inv);
     }
+#pragma unroll
+    for (int s = 0; s < KF; s++) att_q<T>::split(qr[s], mul * a.sign, qf[s]);
+    const float c = a.c * inv;
     while (key0 < k_end) {
         const int32_t next = key0 + stride;
-        f32x4 s[NB][2];
+        f32x4 s[2];
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++)
+        for (int b = 0; b < 2; b++) {
+            s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                s[nb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < KF; i++)
 #pragma unroll
-                for (int i = 0; i < KF; i++)
-#pragma unroll
-                    for (int t = 0; t < NQ; t++) s[nb][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b][i], qf[nb][i][t], s[nb][b], 0, 0, 0);
-            }
+                for (int t = 0; t < NQ; t++) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b][i], qf[i][t], s[b], 0, 0, 0);
+        }
         // (without a condition on there being a next block: behind the last one this reads row 0, and a condition here
         // makes the compiler copy what it loads, that is wait for it)
         const uint32_t nrow = att_row(a, ahead, bad);
@@ -531,35 +517,30 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
         const bool partial = key0 < k_lo || is_partial(key0);  // (a block that ends behind the last key is one)
         if (partial) {
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
+            for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int b = 0; b < 2; b++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int32_t key = key0 + b * 16 + (int32_t)g * 4 + i;
-                        if (key < k_lo || key > pos[nb] || (a.window && key <= pos[nb] - (int32_t)a.window)) s[nb][b][i] = NEG_INF;
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const int32_t key = key0 + b * 16 + (int32_t)g * 4 + i;
+                    if (key < k_lo || key > pos || (a.window && key <= pos - (int32_t)a.window)) s[b][i] = NEG_INF;
+                }
         }
-        f16x8 ph[NB], pl[NB];
+        f16x8 ph, pl;
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = max_xor<32>(max_xor<16>(mx)) * c;
+        if (__any(mx > m + kMaxLag)) {  // the reference is moved on rarely: weights may grow to 2^kMaxLag
+            const float mn = fmaxf(m, mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
+            l *= alpha;
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-            float mx = fmaxf(fmaxf(fmaxf(s[nb][0][0], s[nb][0][1]), fmaxf(s[nb][0][2], s[nb][0][3])), fmaxf(fmaxf(s[nb][1][0], s[nb][1][1]), fmaxf(s[nb][1][2], s[nb][1][3])));
-            mx = max_xor<32>(max_xor<16>(mx)) * c[nb];
-            if (__any(mx > m[nb] + kMaxLag)) {  // the reference is moved on rarely: weights may grow to 2^kMaxLag
-                const float mn = fmaxf(m[nb], mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m[nb] - mn);
-                l[nb] *= alpha;
+            for (int i = 0; i < CH; i++) o[i] *= alpha;
+            m = mn;
+        }
+        const float sub = m == NEG_INF ? 0.f : kProbShift - m;
 #pragma unroll
-                for (int i = 0; i < CH; i++) o[nb][i] *= alpha;
-                m[nb] = mn;
-            }
-            const float sub = m[nb] == NEG_INF ? 0.f : kProbShift - m[nb];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float p = exp2_hw(__builtin_fmaf(s[nb][j >> 2][j & 3], c[nb], sub));
-                l[nb] += p;
-                ph[nb][j] = (f16_t)p;
-                if constexpr (NQ == 2) pl[nb][j] = (f16_t)(p - (float)ph[nb][j]);
-            }
+        for (int j = 0; j < 8; j++) {
+            const float p = exp2_hw(__builtin_fmaf(s[j >> 2][j & 3], c, sub));
+            l += p;
+            ph[j] = (f16_t)p;
+            if constexpr (NQ == 2) pl[j] = (f16_t)(p - (float)ph[j]);
         }
         if (partial) {  // keys that no row sees: zero; values that are not finite: see below
 #pragma unroll
@@ -589,17 +570,15 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
         }
         load_v(nrow);
 #pragma unroll
-        for (int i = 0; i < CH; i++)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                o[nb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], ph[nb], o[nb][i], 0, 0, 0);
-                if constexpr (NQ == 2) o[nb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], pl[nb], o[nb][i], 0, 0, 0);
-            }
+        for (int i = 0; i < CH; i++) {
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], ph, o[i], 0, 0, 0);
+            if constexpr (NQ == 2) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], pl, o[i], 0, 0, 0);
+        }
         key0 = next;
         __builtin_amdgcn_sched_barrier(0);  // V is issued here, not at the head of the next round
     }
     att_report(a, bad);
-    // o[nb][ci][i]: row nb * 16 + n16, channel chan(4 g + i, ci); heads of 256 channels hold two runs of eight, 128 apart
+    // o[ci][i]: row n16, channel chan(4 g + i, ci); heads of 256 channels hold two runs of eight, 128 apart
     auto chan = [&](int i, int ci) { return CH == 16 ? (ci >> 3) * 128 + ((int)g * 4 + i) * 8 + (ci & 7) : ((int)g * 4 + i) * CH + ci; };
     // A value of V that is not finite, in a block that some rows see only in part, was cleared on its way in, so that it
     // met no weight of zero; the rows that do see it get it here, as it is (any weight above zero leaves it so).
@@ -617,33 +596,27 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
                     for (int ci = 0; ci < CH; ci++) {
                         const float x = (float)p[chan(i, ci)];
                         const bool nonfinite = !(__builtin_fabsf(x) < __builtin_inff());
-#pragma unroll
-                        for (int nb = 0; nb < NB; nb++)
-                            if (nonfinite && key <= pos[nb] && !(a.window && key <= pos[nb] - (int32_t)a.window)) o[nb][ci][i] += x;
+                        if (nonfinite && key <= pos && !(a.window && key <= pos - (int32_t)a.window)) o[ci][i] += x;
                     }
             }
         }
     }
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++) l[nb] = sum_xor<32>(sum_xor<16>(l[nb]));
+    l = sum_xor<32>(sum_xor<16>(l));
     float* part = att_part(a, split ? slot : 0, kvh);
     if (WK == 1) {  // a wave has the whole result of its head
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-            const uint32_t r = nb * 16 + n16;
-            if (r >= rows_here) continue;
-            const float f = split ? 1.f : att_inverse(l[nb]);
+        if (on) {
+            const float f = split ? 1.f : att_inverse(l);
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int ci = 0; ci < CH; ci += 4) {
-                    float t[4] = {o[nb][ci][i] * f, o[nb][ci + 1][i] * f, o[nb][ci + 2][i] * f, o[nb][ci + 3][i] * f};
-                    if (split) io<float>::store(part + (uint64_t)r * HD + chan(i, ci), t);
-                    else att_store4<T>((T*)a.out + qat[nb] + chan(i, ci), t);
+                    float t[4] = {o[ci][i] * f, o[ci + 1][i] * f, o[ci + 2][i] * f, o[ci + 3][i] * f};
+                    if (split) io<float>::store(part + (uint64_t)n16 * HD + chan(i, ci), t);
+                    else att_store4<T>((T*)a.out + qat + chan(i, ci), t);
                 }
             if (split && g == 0) {
-                part[R * HD + r] = m[nb];
-                part[R * (HD + 1) + r] = l[nb];
+                part[R * HD + n16] = m;
+                part[R * (HD + 1) + n16] = l;
             }
         }
         continue;
@@ -654,25 +627,19 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     float* sm_l = smem + W * R;      // [W][R]
     float* sm_o = smem + 2 * W * R;  // [W][RR][HD]
     const uint32_t hl = wave % a.heads;  // the head's waves: hl, hl + heads, ...
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++)
-        if (g == 0) sm_m[wave * R + nb * 16 + n16] = m[nb];
+    if (g == 0) sm_m[wave * R + n16] = m;
     __syncthreads();
+    float M = NEG_INF;
+    for (uint32_t w = hl; w < W; w += a.heads) M = fmaxf(M, sm_m[w * R + n16]);
+    const float f = m == NEG_INF ? 0.f : exp2_hw(m - M);
+    if (g == 0) sm_l[wave * R + n16] = l * f;
+    if (on) {
+        float* dst = sm_o + ((uint64_t)wave * RR + n16) * HD;
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        const uint32_t r = nb * 16 + n16;
-        float M = NEG_INF;
-        for (uint32_t w = hl; w < W; w += a.heads) M = fmaxf(M, sm_m[w * R + r]);
-        const float f = m[nb] == NEG_INF ? 0.f : exp2_hw(m[nb] - M);
-        if (g == 0) sm_l[wave * R + r] = l[nb] * f;
-        if (r < RR) {
-            float* dst = sm_o + ((uint64_t)wave * RR + r) * HD;
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int ci = 0; ci < CH; ci += 4)
-                    *(f32x4*)(dst + chan(i, ci)) = f32x4{o[nb][ci][i] * f, o[nb][ci + 1][i] * f, o[nb][ci + 2][i] * f, o[nb][ci + 3][i] * f};
-        }
+            for (int ci = 0; ci < CH; ci += 4)
+                *(f32x4*)(dst + chan(i, ci)) = f32x4{o[ci][i] * f, o[ci + 1][i] * f, o[ci + 2][i] * f, o[ci + 3][i] * f};
     }
     __syncthreads();
     const uint32_t kvh0 = blockIdx.x % hblocks * a.heads;
@@ -703,21 +670,16 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     }
 }
 extern __shared__ float att_smem[];
-#define ATTEND_FEW(HD, NB, W)                                                                                                \
-    extern "C" __global__ __launch_bounds__(W * 64, W / 4) void apk_attend_few_f16_hd##HD##_b##NB(apk_attend_args a) {       \
-        attend_few_body<f16_t, HD, NB, W>(a, att_smem);                                                                      \
-    }                                                                                                                        \
-    extern "C" __global__ __launch_bounds__(W * 64, W / 4) void apk_attend_few_f32_hd##HD##_b##NB(apk_attend_args a) {       \
-        attend_few_body<float, HD, NB, W>(a, att_smem);                                                                      \
+#define ATTEND_FEW(HD, W)                                                                                          \
+    extern "C" __global__ __launch_bounds__(W * 64, W / 4) void apk_attend_few_f16_hd##HD(apk_attend_args a) {     \
+        attend_few_body<f16_t, HD, W>(a, att_smem);                                                                \
+    }                                                                                                              \
+    extern "C" __global__ __launch_bounds__(W * 64, W / 4) void apk_attend_few_f32_hd##HD(apk_attend_args a) {     \
+        attend_few_body<float, HD, W>(a, att_smem);                                                                \
     }
-ATTEND_FEW(64, 1, 8)
-ATTEND_FEW(64, 2, 8)
-ATTEND_FEW(64, 4, 8)
-ATTEND_FEW(128, 1, 8)
-ATTEND_FEW(128, 2, 8)
-ATTEND_FEW(128, 4, 4)
-ATTEND_FEW(256, 1, 4)
-ATTEND_FEW(256, 2, 4)
+ATTEND_FEW(64, 8)
+ATTEND_FEW(128, 8)
+ATTEND_FEW(256, 4)
 
 // ------------------------------------------------------------------------------------------- chunks of new tokens
 // One workgroup of four waves per (sequence, kv head, tile of 128 flat (token, head) rows, part of the keys); a wave holds 32
