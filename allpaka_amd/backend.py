@@ -731,6 +731,7 @@ class PagedCache:
     def extend(self, n_new, rows, step=None):
         """n_new int32 [n_seq] more tokens; rows: the most there can be in all.  Shared pages that get written to are copied
         in every plane.  Returns the PageStep (step: one to fill, of this n_seq and rows)."""
+        assert step is not None or not self.b._recording, "a recording needs a step that outlives it"
         step = PageStep(self.n_seq, rows, self.b.device) if step is None else step
         assert step.rows == rows and step.n_seq == self.n_seq
         self.b._order()

@@ -4,7 +4,7 @@
 #include <stdint.h>
 
 // Rows of a tile of the chunk kernel: flat (token, head of the group) rows of one kv head.  (The kernel for few rows takes
-// 16, 32 or 64.)
+// 16.)
 #define APK_ATT_CHUNK_ROWS 128u
 // The scratch: one word, the number of tiles listed; from word 16 on 8 words for each of them (first row and rows of the
 // sequence, tile, parts, slots of the first and the second part and the step to the next ones); from APK_ATT_PART_AT bytes

@@ -226,6 +226,8 @@ DEV uint32_t att_share(const apk_attend_args& a, uint32_t w, uint64_t& x0, uint6
     // (32-bit division where the numbers allow it)
     share = all < 0x80000000u ? ((uint32_t)all + a.target - 1) / a.target : (all + a.target - 1) / a.target;
     if (share < a.unit_min) share = a.unit_min;
+    // (no tile is ever cut there, also where wrong row offsets make more tiles than the launch has workgroups)
+    if (a.whole_units) share = (share + a.whole_units - 1) / a.whole_units * a.whole_units;
     x0 = min(all, share * w);
     x1 = min(all, x0 + share);
     return tiles;
@@ -775,7 +777,9 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         });
     };
     // some row of the tile does not see all keys of this unit
-    auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
+    // (the unit behind an odd last one of a part is the next part's: no key of it counts here)
+    const int32_t part_end = (int32_t)(sp.u1 * BN), pos_end = min(pos, part_end - 1);
+    auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > min(tpos0, part_end - 1) || (a.window && key0 <= tpos1 - (int32_t)a.window); };
     f16x8 qf[KF][NQ];
     float c = a.c;
     {
@@ -900,7 +904,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const int32_t key = key0 + b * 32 + 8 * (j >> 2) + 4 * (int32_t)hf + (j & 3);
-            if (key > pos || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
+            if (key > pos_end || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
         }
     };
     // A unit that all rows see whole, in buffer `buf`.  Blocks of 32 keys, so that a wave has products and softmax to run

@@ -433,3 +433,50 @@ def test_refusals(be):
         with pytest.raises(C.ArgumentError):
             call(False, **bad)
     assert be.take_faults() == 0
+
+
+# chunks over long caches, whose tiles are cut into few and into many parts; groups of more heads than a tile of few rows
+LONG = [
+    # (cached, new) each, n_q, n_kv, hd, page, window
+    ([(9000, 40)], 6, 2, 128, 64, 0),
+    ([(20000, 5), (30, 30)], 8, 1, 64, 16, 0),
+    ([(7000, 30), (100, 2)], 4, 1, 256, 33, 0),
+    ([(6000, 200)], 3, 1, 128, 16, 4000),
+    ([(5000, 33), (0, 150), (700, 1)], 9, 3, 64, 24, 0),
+    ([(3000, 70)], 6, 2, 256, 16, 700),
+    ([(4000, 1), (2500, 1)], 40, 2, 128, 16, 0),
+    ([(900, 1), (3, 1)], 100, 1, 256, 16, 0),
+]
+
+
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("i", range(len(LONG)))
+def test_chunks_over_long_caches(be, i, f16):
+    seqs, n_q, n_kv, hd, page, window = LONG[i]
+    c = make_case(600 + i, [a + b for a, b in seqs], [b for _, b in seqs], n_q, n_kv, hd, page, f16)
+    want, tol = attention64(c, hd ** -0.5, window)
+    close(run(be, c, hd ** -0.5, window), want, tol, "chunk entry")
+    if all(b == 1 for _, b in seqs):
+        close(run(be, c, hd ** -0.5, window, chunk=False), want, tol, "token entry")
+
+
+def test_row_offsets_that_name_rows_twice(be):
+    """A descending pair between two ascending ones: more tiles than the rows make.  The call reports it and ends, and rows
+    behind are left as they are."""
+    import allpaka_amd.lib as apklib
+
+    for hd in (64, 128, 256, 32):
+        for lens in ([40, 50, 60], [3000, 50, 2000]):
+            c = make_case(620, lens, [4, 0, 0], 16, 1, hd, 16, True, garbage=0.0)
+            out = torch.full((4, 16 * hd), 5.0, dtype=torch.float16, device="cuda")
+            be.attend_paged_chunk_into(dev(c["q"]), dev(c["K"]), dev(c["V"]), 16, dev(c["table"]), dev(np.array([0, 4, 0, 4], np.int32)),
+                                       dev(c["kv_len"]), 16, 1, hd, 0.1, out)
+            assert be.take_faults() & apklib.FAULT_ROW_RANGE
+
+
+def test_heads_that_are_no_power_of_two(be):
+    for n_kv, group in ((3, 5), (6, 1), (7, 2)):
+        for chunk in (False, True):
+            c = make_case(630 + n_kv, [1500, 33, 700], [9, 1, 4] if chunk else [1, 1, 1], n_kv * group, n_kv, 128, 16, True)
+            want, tol = attention64(c, 0.09)
+            close(run(be, c, 0.09, chunk=chunk), want, tol, f"{n_kv} kv heads")

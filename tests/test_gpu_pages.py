@@ -364,3 +364,35 @@ def test_a_serving_run(be, ora):
     one([1, 6, 1, 1], rec.graph.launch)
     one([2, 1, 0, 3], enqueue)
     rec.graph.destroy()
+
+
+def test_more_new_pages_in_one_step_than_fit_on_the_chip(be):
+    """Thousands of pages taken by one call, by one sequence and by many."""
+    for n_seq, new in ((1, [9000]), (3, [1, 4096, 4500]), (2000, [5] * 2000)):
+        page = 1 if n_seq < 2000 else 2
+        cache, model = new_cache(be, 12000, page, n_seq, 10000 if n_seq < 2000 else 8, width=8), PageModel(12000, page, n_seq, 10000 if n_seq < 2000 else 8)
+        rows = sum(new) + 3
+        step = cache.extend(i32(new), rows)
+        assert be.take_faults() == 0
+        check_step(step, model.extend(new, rows), rows)
+        same(cache, model)
+        step = cache.extend(i32([1] * n_seq), n_seq)
+        check_step(step, model.extend([1] * n_seq, n_seq), n_seq)
+        same(cache, model)
+
+
+def test_saved_and_restored(be):
+    cache, model = new_cache(be, 40, 4, 3, 8), PageModel(40, 4, 3, 8)
+    cache.extend(i32([5, 9, 0]), 14)
+    model.extend([5, 9, 0], 14)
+    saved = cache.save()
+    cache.truncate(i32([0, 2, -1]))
+    cache.extend(i32([1, 1, 7]), 9)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        cache.restore(saved)
+    be.sync()
+    same(cache, model)
+    with pytest.raises(AssertionError):
+        cache.restore(saved[:-4])
+    assert be.take_faults() == 0
