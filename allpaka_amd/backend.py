@@ -628,34 +628,39 @@ class PageStep:
 
     def __init__(self, n_seq, rows, device):
         self.n_seq, self.rows = n_seq, rows
-        # one buffer: q_off [n_seq + 1], positions [rows], slots [rows], the pairs [n_seq, 2] copied and their number
-        self._buf = torch.empty(n_seq + 1 + 2 * rows + 2 * n_seq + 1, dtype=torch.int32, device=device)
-        at = self._buf.data_ptr()
-        sizes = (n_seq + 1, rows, rows, 2 * n_seq, 1)
-        self._ptrs = [at + 4 * sum(sizes[:i]) for i in range(5)]
+        # one buffer of parts that begin at whole 16-byte tiles
+        self._at, total = [], 0
+        for size in (n_seq + 1, rows, rows, 2 * n_seq, 1):
+            self._at.append((total, size))
+            total += (size + 3) // 4 * 4
+        self._buf = torch.empty(total, dtype=torch.int32, device=device)
+        self._ptrs = [self._buf.data_ptr() + 4 * at for at, _ in self._at]
+
+    def _part(self, i):
+        at, size = self._at[i]
+        return self._buf[at:at + size]
 
     @property
     def q_off(self):
-        return self._buf[:self.n_seq + 1]
+        return self._part(0)
 
     @property
     def positions(self):
-        return self._buf[self.n_seq + 1:self.n_seq + 1 + self.rows]
+        return self._part(1)
 
     @property
     def slots(self):
-        return self._buf[self.n_seq + 1 + self.rows:self.n_seq + 1 + 2 * self.rows]
+        return self._part(2)
 
     @property
     def pairs(self):
         """(to, from) of the pages that were copied, the first n_pairs of them."""
-        at = self.n_seq + 1 + 2 * self.rows
-        return self._buf[at:at + 2 * self.n_seq].view(self.n_seq, 2)
+        return self._part(3).view(self.n_seq, 2)
 
     @property
     def n_pairs(self):
         """The number of pages that were copied."""
-        return self._buf[-1:]
+        return self._part(4)
 
 
 class PagedCache:
@@ -670,12 +675,13 @@ class PagedCache:
         self.n_pages, self.n_seq, self.max_pages = region.shape[1] // page_size, n_seq, max_pages
         dev = backend.device
         words = backend.L.apk_pages_words(self.n_pages)
-        # one buffer of whole 16-byte tiles, so that the state is saved and restored by one copy
-        total = words + n_seq * max_pages + n_seq
-        self._all = torch.zeros((total + 3) // 4 * 4, dtype=torch.int32, device=dev)
+        # one buffer, so that the state is saved and restored by one copy; its parts begin at whole 16-byte tiles
+        table = (words + 3) // 4 * 4
+        lens = table + (n_seq * max_pages + 3) // 4 * 4
+        self._all = torch.zeros(lens + (n_seq + 3) // 4 * 4, dtype=torch.int32, device=dev)
         self.pool = self._all[:words]
-        self.page_table = self._all[words:words + n_seq * max_pages].view(n_seq, max_pages)
-        self.kv_len = self._all[total - n_seq:total]
+        self.page_table = self._all[table:table + n_seq * max_pages].view(n_seq, max_pages)
+        self.kv_len = self._all[lens:lens + n_seq]
         self.page_table.fill_(-1)
         self._moves = torch.empty((max(self.n_pages // 2, 1), 2), dtype=torch.int32, device=dev)
         self._n_moves = torch.zeros(1, dtype=torch.int32, device=dev)

@@ -386,7 +386,9 @@ DEV u32x4 att_clear_nonfinite(u32x4 t) {
 // cache where there are W heads or more, and its waves need not be joined.  K and V go from memory straight to registers:
 // a wave's K block is the first operand of 16x16x32 products as it lies (16 bytes of a key a lane), its V block becomes
 // one by an in-lane transpose (8 keys x 8 channels a lane).  K of the next block is under way from the moment K of this
-// one is used up, V likewise.  Bound by the stream of K and V.
+// one is used up, V likewise.  Bound by the stream of K and V: 131071 keys of 8 heads of 128 in 96 us (5.6 TB/s), 64
+// sequences of 100 to 12000 keys in 280 us (5.8 TB/s), where reads in this pattern without any arithmetic reach 5.9 to
+// 6.2.  Short caches are bound by the chain launch, length, table entry, K, V, joins: 13 us for 600 keys.
 template <typename T, int HD, int W>
 DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     constexpr int KF = HD / 32;           // K fragments of 16 keys
@@ -689,6 +691,11 @@ ATTEND_FEW(256, 4)
 // buffers while the unit in the other is worked on; one barrier a unit.  K rows are the first operand of 32x32x16 products
 // as they lie; V comes out of LDS transposed (ds_read_b64_tr_b16), in the key order in which a lane holds its
 // probabilities.  The 16-byte chunks of LDS row r are permuted by f(r), so that both kinds of reads meet all banks.
+// Bound by the three that do not overlap fully, matrix instructions, LDS reads and exponentials, each near 2000 cycles for
+// the units that the two workgroups of a CU (one for f32 heads of 128 and heads of 256) work on together: 512 tokens over
+// 32000 keys, 64 / 8 heads of 128, fp16: 595 us, 0.9 PFLOP/s, where a large matrix product reaches 1.3; without the loads
+// 15 % less, without the exponentials 17 % less.  64 rows a wave read LDS half as often, but leave one wave per SIMD,
+// whose products and exponentials then wait for each other: 760 us.
 template <int HD> DEV uint32_t att_swz(uint32_t r) {
     if constexpr (HD == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
     else return ((r & 3) << 2) | ((r >> 2) & 3);
@@ -741,12 +748,15 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     const uint32_t flat = flat0 + wave * 32 + n32;
     const bool on = flat < flat_n;
     const uint32_t tok = flat / a.group, head = flat % a.group;
-    const int32_t pos = on ? it.s.p0 + (int32_t)tok : -1;
-    const int32_t pos_lo = a.window ? pos - (int32_t)a.window : -1;  // keys above this one
+    // (no key behind the part counts: heads of 256 go through units in pairs, and the one behind an odd last one is the
+    // next part's)
+    const int32_t part_last = (int32_t)(sp.u1 * BN) - 1, row_pos = it.s.p0 + (int32_t)tok;
+    const int32_t pos = on ? min(row_pos, part_last) : -1;
+    const int32_t pos_lo = a.window ? row_pos - (int32_t)a.window : -1;  // keys above this one
     const bool wave_on = flat0 + wave * 32 < flat_n;
     const int32_t wpos0 = it.s.p0 + uni((int32_t)((flat0 + wave * 32) / a.group));
     const int32_t wpos1 = it.s.p0 + uni((int32_t)((min(flat0 + wave * 32 + 32, flat_n) - 1) / a.group));
-    const int32_t tpos0 = it.s.p0 + (int32_t)tok0, tpos1 = it.s.p0 + (int32_t)tok1;
+    const int32_t tpos0 = min(it.s.p0 + (int32_t)tok0, part_last), tpos1 = it.s.p0 + (int32_t)tok1;
     const uint64_t qat = ((uint64_t)(it.s.row0 + tok) * a.n_q + kvh * a.group + head) * HD;
 
     // staging: thread t takes chunks t, t + 256, ... of a unit.  A lane looks one key up, a unit ahead; rows are handed round.
@@ -777,9 +787,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         });
     };
     // some row of the tile does not see all keys of this unit
-    // (the unit behind an odd last one of a part is the next part's: no key of it counts here)
-    const int32_t part_end = (int32_t)(sp.u1 * BN), pos_end = min(pos, part_end - 1);
-    auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > min(tpos0, part_end - 1) || (a.window && key0 <= tpos1 - (int32_t)a.window); };
+    auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
     f16x8 qf[KF][NQ];
     float c = a.c;
     {
@@ -904,10 +912,10 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const int32_t key = key0 + b * 32 + 8 * (j >> 2) + 4 * (int32_t)hf + (j & 3);
-            if (key > pos_end || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
+            if (key > pos || (a.window && key <= pos_lo)) s[b][j] = NEG_INF;
         }
     };
-    // A unit that all rows see whole, in buffer `buf`.  Blocks of 32 keys, so that a wave has products and softmax to run
+    // A unit in buffer `buf`; unless ANY, one that all rows see whole.  Blocks of 32 keys, so that a wave has products and softmax to run
     // side by side: the products of block 1's scores next to block 0's exponentials, those of block 0's values next to
     // block 1's; LDS reads stand a few products before their use.  (fetch: behind the last unit it reads row 0, which is
     // not used; a condition would make the compiler wait for the table entries.)
@@ -1009,7 +1017,9 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     uint32_t f0 = max(sp.u0, (uint32_t)max(0, (max(w0, sp.lo) + BN - 1) / BN)), f1 = min(sp.u1, (uint32_t)max(0, w1 / BN));
     f0 = min(f0, sp.u1);
     f1 = f1 > f0 && wave_on ? f0 + ((f1 - f0) & ~1u) : f0;
-    constexpr bool ONE = HD == 256;  // two such bodies do not fit the registers: one for all units, in pairs from the first
+    // Heads of 256: two such bodies do not fit the registers (5 chunks of 333 to 2500 tokens: 608 us; 32 keys at a time, with
+    // nothing side by side, 429), so one serves all units, in pairs from the first (318 us).
+    constexpr bool ONE = HD == 256;
     const uint32_t parity = ONE ? sp.u0 & 1 : f0 & 1;
     if (sp.u0 < sp.u1) {
         look(sp.u0);
@@ -1101,7 +1111,8 @@ ATTEND_CHUNK(float, f32, 128, 64, 1)
 ATTEND_CHUNK(float, f32, 256, 64, 1)
 
 // ------------------------------------------------------------------------------------------- joining the parts
-// The tiles that were cut: a workgroup of eight waves takes join_rows rows of one listed tile and kv head.  Of up
+// The tiles that were cut: a workgroup of eight waves takes join_rows rows of one listed tile and kv head.  Bound by the
+// round trips of the parts' loads, 4 us where little was cut, 15 for 256 tiles of 128 rows in two parts (34 MB).  Of up
 // to 32 parts a wave joins a row on its own, hd / 4 lanes to a part; of more the whole workgroup shares the parts of one
 // row after the other, so that the loads of all of them are under way together.
 template <typename T>
