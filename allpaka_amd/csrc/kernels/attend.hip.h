@@ -866,12 +866,19 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b][q], o[hb], 0, 0, 0);
         if constexpr (NQ == 2) o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b][q], o[hb], 0, 0, 0);
     };
-    auto weight = [&](int b, int j, float sub) {
-        const float p = exp2_hw(__builtin_fmaf(s[b][j], c, sub));
-        l += p;
-        const f16_t h = (f16_t)p;
-        ph[b][j >> 3][j & 7] = h;
-        if constexpr (NQ == 2) pl[b][j >> 3][j & 7] = (f16_t)(p - (float)h);
+    auto weight = [&](int b, int j, float sub) {  // the block's scores 2 j and 2 j + 1
+        const f32x2 p = {exp2_hw(__builtin_fmaf(s[b][2 * j], c, sub)), exp2_hw(__builtin_fmaf(s[b][2 * j + 1], c, sub))};
+        l += p.x;
+        l += p.y;
+        const f16x2 h = __builtin_convertvector(p, f16x2);
+        ph[b][j >> 2][2 * j & 7] = h.x;
+        ph[b][j >> 2][(2 * j & 7) + 1] = h.y;
+        if constexpr (NQ == 2) {
+            const f32x2 d = {__builtin_fmaf((float)h.x, -1.f, p.x), __builtin_fmaf((float)h.y, -1.f, p.y)};
+            const f16x2 e = __builtin_convertvector(d, f16x2);
+            pl[b][j >> 2][2 * j & 7] = e.x;
+            pl[b][j >> 2][(2 * j & 7) + 1] = e.y;
+        }
     };
     auto shift = [&]() { return m == NEG_INF ? 0.f : kProbShift - m; };
     auto values = [&](int b, uint32_t v_at) {
@@ -969,7 +976,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             if (i + AHEAD < KF) kf[i + AHEAD] = load_k(1, i + AHEAD, k_at);
             score(1, i, kf[i]);
 #pragma unroll
-            for (int j = i * 16 / KF; j < (i + 1) * 16 / KF; j++) weight(0, j, sub);
+            for (int j = i * 8 / KF; j < (i + 1) * 8 / KF; j++) weight(0, j, sub);
             __builtin_amdgcn_sched_barrier(0);
         }
         f16x8 vf[2][2];
@@ -980,7 +987,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             l = before * alpha;
             sub = shift();
 #pragma unroll
-            for (int j = 0; j < 16; j++) weight(0, j, sub);
+            for (int j = 0; j < 8; j++) weight(0, j, sub);
         });
         sub = shift();
         __builtin_amdgcn_sched_barrier(0);
@@ -998,7 +1005,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
                     if (b == 0) {
                         const int x = hb * 2 + q;
 #pragma unroll
-                        for (int j = x * 16 / (2 * HB); j < (x + 1) * 16 / (2 * HB); j++) weight(1, j, sub);
+                        for (int j = x * 8 / (2 * HB); j < (x + 1) * 8 / (2 * HB); j++) weight(1, j, sub);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -1022,7 +1029,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
                 refer(b, [&](float alpha) { l *= alpha; });
                 const float sub = shift();
 #pragma unroll
-                for (int j = 0; j < 16; j++) weight(b, j, sub);
+                for (int j = 0; j < 8; j++) weight(b, j, sub);
                 values(b, (2 + buf) * BUF);
             }
         }
