@@ -866,6 +866,8 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b][q], o[hb], 0, 0, 0);
         if constexpr (NQ == 2) o[hb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b][q], o[hb], 0, 0, 0);
     };
+    float neg = -1.f;  // hidden from the compiler, which then takes a fp16 factor into one instruction with the subtraction
+    asm("" : "+v"(neg));
     auto weight = [&](int b, int j, float sub) {  // the block's scores 2 j and 2 j + 1
         const f32x2 p = {exp2_hw(__builtin_fmaf(s[b][2 * j], c, sub)), exp2_hw(__builtin_fmaf(s[b][2 * j + 1], c, sub))};
         l += p.x;
@@ -874,7 +876,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         ph[b][j >> 2][2 * j & 7] = h.x;
         ph[b][j >> 2][(2 * j & 7) + 1] = h.y;
         if constexpr (NQ == 2) {
-            const f32x2 d = {__builtin_fmaf((float)h.x, -1.f, p.x), __builtin_fmaf((float)h.y, -1.f, p.y)};
+            const f32x2 d = {__builtin_fmaf((float)h.x, neg, p.x), __builtin_fmaf((float)h.y, neg, p.y)};
             const f16x2 e = __builtin_convertvector(d, f16x2);
             pl[b][j >> 2][2 * j & 7] = e.x;
             pl[b][j >> 2][(2 * j & 7) + 1] = e.y;
