@@ -1836,7 +1836,7 @@ int apk_pages_copy(apk_ctx* c, void* region, size_t n_planes, size_t plane_bytes
     uint32_t np = (uint32_t)n_pages, npl = (uint32_t)n_planes, mp = (uint32_t)max_pairs;
     uint64_t plb = plane_bytes, pgb = page_bytes;
     const uint64_t tiles = page_bytes / 16;
-    uint32_t slices = (uint32_t)((tiles + 1023) / 1024), span = (uint32_t)((tiles + slices - 1) / slices);
+    uint32_t slices = (uint32_t)((tiles + 2047) / 2048), span = (uint32_t)((tiles + slices - 1) / slices);
     if (max_pairs > 0xffffffffu / slices) return fail(APK_DECLINE_SHAPE, "apk_pages_copy: too large");
     const double items = (double)max_pairs * (double)n_planes * slices;
     const unsigned grid = items < 8192. ? (unsigned)items : 8192u;

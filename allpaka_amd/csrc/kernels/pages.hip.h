@@ -525,11 +525,11 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_compact_k(uint3
 }
 
 // Page pairs[2 i + 1] copied over page pairs[2 i] in every plane, *n_pairs of them (at most max_pairs).  An item is one slice
-// (span tiles of 16 bytes, no more than 4 per lane) of one pair in one plane; workgroups take items in turn, plane after
+// (span tiles of 16 bytes, no more than 8 per lane) of one pair in one plane; workgroups take items in turn, plane after
 // plane.  Bound by memory: a plain copy whose addresses come out of a list.  1.2 GB in pages of 32 KiB move in 235 us
-// (5.3 TB/s, a copy of one piece 6.7).  The reads stay in the caches: 32 copies of one shared page in 64 planes take 33 us,
-// 60 with reads marked as not to be kept, which move distinct pages in 230; planes side by side instead of one after the
-// other take 250.
+// (5.3 TB/s, a copy of one piece 6.7).  The reads stay in the caches: 32 copies of one shared page in 64 planes take 27 us
+// (33 with 4 tiles a lane), twice that with reads marked as not to be kept, which move distinct pages in 230; planes side
+// by side instead of one after the other take 250.
 extern "C" __global__ __launch_bounds__(256) void apk_pages_copy_k(char* region, uint32_t n_planes, uint64_t plane_bytes, uint32_t n_pages,
                                                                    uint64_t page_bytes, const uint32_t* pairs, const uint32_t* n_pairs,
                                                                    uint32_t max_pairs, uint32_t slices, uint32_t span, uint32_t* fault) {
@@ -554,12 +554,12 @@ extern "C" __global__ __launch_bounds__(256) void apk_pages_copy_k(char* region,
         }
         const u32x4* src = (const u32x4*)(base + from * page_bytes);
         char* dst = base + to * page_bytes;
-        u32x4 v[4];
+        u32x4 v[8];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 8; k++)
             v[k] = src[t0 + k * 256 < t1 ? t0 + k * 256 : 0];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 8; k++)
             if (t0 + k * 256 < t1) nt_store(v[k], dst + (uint64_t)(t0 + k * 256) * 16);
     }
 }
