@@ -33,6 +33,6 @@ struct apk_attend_args {
     uint32_t join_rows;       // rows that a workgroup of the joining launch takes
     uint32_t tile_rows, unit; // rows of a tile and keys of a unit, powers of two, and their logarithms
     uint32_t tile_shift, unit_shift;
-    float c;                  // |scale| * log2(e), kept above zero
-    float sign;               // the sign of scale, applied to q
+    float scale;              // its magnitude
+    float sign;               // and its sign, applied to q
 };

@@ -1623,7 +1623,7 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
     a.max_pages = (uint32_t)max_pages;
     a.n_pages = (uint32_t)(capacity / page_size);
     a.window = window >= max_pages * page_size ? 0 : (uint32_t)window;
-    a.c = fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f);  // above zero: a masked score stays -inf when multiplied by it
+    a.scale = fabsf(scale);
     a.sign = scale < 0.f ? -1.f : 1.f;
     const std::string t_name = dtype == APK_F32 ? "f32" : "f16";
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) {

@@ -24,7 +24,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-static constexpr float kProbShift = 8.0f, kMaxLag = 7.0f;
+static constexpr float kProbShift = 8.0f, kMaxLag = 7.0f, kLog2e = 1.44269504088896341f;
 #define NEG_INF (-__builtin_inff())
 
 // {lane's own value, that of lane ^ X} in some order, X = 16 or 32: one swap of half rows, no LDS.  Written out, because
@@ -359,14 +359,21 @@ template <> struct att_q<float> {
         }
     }
 };
-// The power of two that brings a row's largest magnitude to [2^13, 2^14), and its inverse; 1 for a row of zeros.
+// The power of two that brings a row's largest magnitude to [2^13, 2^14) or, for the smallest ones, as near as 2^126 does,
+// and its inverse; 1 for a row that is not finite.
 DEV void att_q_scale(float mx, float& mul, float& inv) {
     const int e = (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 0xff);  // biased exponent
     int k = 127 + 13 - e;                                                  // multiply by 2^k
-    if (e == 0 || e == 255) k = 0;
+    if (e == 255) k = 0;
     k = k > 126 ? 126 : k < -126 ? -126 : k;
     mul = __builtin_bit_cast(float, (uint32_t)(127 + k) << 23);
     inv = __builtin_bit_cast(float, (uint32_t)(127 - k) << 23);
+}
+// What a row's products are multiplied by: |scale| * log2(e) / its power of two, the exact product first, so that a scale and
+// a row whose sizes undo each other lose nothing.  Kept a normal number: a masked score stays -inf when multiplied by it
+// (with 0 it would be NaN), and a score of 0 stays 0.  The least one moves no weight: a row's products are below 2^40.
+DEV float att_factor(const apk_attend_args& a, float inv) {
+    return __builtin_amdgcn_fmed3f(a.scale * inv * kLog2e, __FLT_MIN__, __FLT_MAX__);
 }
 
 template <typename T> DEV void att_store8(T* p, const float* v);
@@ -516,7 +523,7 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     }
 #pragma unroll
     for (int s = 0; s < KF; s++) att_q<T>::split(qr[s], mul * a.sign, qf[s]);
-    const float c = a.c * inv;
+    const float c = att_factor(a, inv);
     while (key0 < k_end) {
         const int32_t next = key0 + stride;
         f32x4 s[2];
@@ -805,7 +812,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     // some row of the tile does not see all keys of this unit
     auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
     f16x8 qf[KF][NQ];
-    float c = a.c;
+    float c;
     {
         typename att_q<T>::raw_t qr[KF];
         float mul = 1.f, inv = 1.f;
@@ -819,7 +826,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         }
 #pragma unroll
         for (int s = 0; s < KF; s++) att_q<T>::split(qr[s], mul * a.sign, qf[s]);
-        c *= inv;
+        c = att_factor(a, inv);
     }
     f32x16 o[HB];
 #pragma unroll
@@ -1288,7 +1295,8 @@ DEV void attend_generic_body(const apk_attend_args& a, float* smem) {
     float* sq = smem;             // [hd]
     float* so = smem + hd;        // [4][hd]
     float* sml = smem + 5 * hd;   // [4][2]
-    for (uint32_t i = threadIdx.x; i < hd; i += 256) sq[i] = (float)((const T*)a.q)[qat + i] * a.sign;
+    // (the scale goes into the query, so that no sum leaves the range that its score has)
+    for (uint32_t i = threadIdx.x; i < hd; i += 256) sq[i] = (float)((const T*)a.q)[qat + i] * a.sign * a.scale;
     __syncthreads();
     float o[16];
 #pragma unroll
@@ -1303,7 +1311,7 @@ DEV void attend_generic_body(const apk_attend_args& a, float* smem) {
             float d = 0.f;
             const f16_t* kr = kb + (uint64_t)r * kv_stride;
             for (uint32_t i = 0; i < hd; i++) d = __builtin_fmaf((float)kr[i], sq[i], d);
-            x = d * a.c;
+            x = d * kLog2e;
         }
         const float mn = fmaxf(m, wave_max_f32(x)), ms = mn == NEG_INF ? 0.f : mn;
         const float alpha = exp2_hw(m - ms), p = exp2_hw(x - ms);
