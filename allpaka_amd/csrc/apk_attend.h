@@ -35,4 +35,5 @@ struct apk_attend_args {
     uint32_t tile_shift, unit_shift;
     float scale;              // its magnitude
     float sign;               // and its sign, applied to q
+    float c;                  // scale * log2(e), kept a normal number: what fp16 rows' products are multiplied by
 };

@@ -15,6 +15,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <map>
@@ -1624,6 +1625,7 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
     a.n_pages = (uint32_t)(capacity / page_size);
     a.window = window >= max_pages * page_size ? 0 : (uint32_t)window;
     a.scale = fabsf(scale);
+    a.c = fminf(fmaxf(a.scale * 1.44269504088896341f, FLT_MIN), FLT_MAX);
     a.sign = scale < 0.f ? -1.f : 1.f;
     const std::string t_name = dtype == APK_F32 ? "f32" : "f16";
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) {

@@ -369,9 +369,10 @@ DEV void att_q_scale(float mx, float& mul, float& inv) {
     mul = __builtin_bit_cast(float, (uint32_t)(127 + k) << 23);
     inv = __builtin_bit_cast(float, (uint32_t)(127 - k) << 23);
 }
-// What a row's products are multiplied by: |scale| * log2(e) / its power of two, the exact product first, so that a scale and
+// What an f32 row's products are multiplied by: |scale| * log2(e) / its power of two, the exact product first, so that a scale and
 // a row whose sizes undo each other lose nothing.  Kept a normal number: a masked score stays -inf when multiplied by it
 // (with 0 it would be NaN), and a score of 0 stays 0.  The least one moves no weight: a row's products are below 2^40.
+// (fp16 rows are not scaled: theirs is a.c, one number that stays in a scalar register.)
 DEV float att_factor(const apk_attend_args& a, float inv) {
     return __builtin_amdgcn_fmed3f(a.scale * inv * kLog2e, __FLT_MIN__, __FLT_MAX__);
 }
@@ -523,7 +524,7 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
     }
 #pragma unroll
     for (int s = 0; s < KF; s++) att_q<T>::split(qr[s], mul * a.sign, qf[s]);
-    const float c = att_factor(a, inv);
+    const float c = NQ == 2 ? att_factor(a, inv) : a.c;
     while (key0 < k_end) {
         const int32_t next = key0 + stride;
         f32x4 s[2];
@@ -812,7 +813,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
     // some row of the tile does not see all keys of this unit
     auto is_partial = [&](int32_t key0) { return key0 + BN - 1 > tpos0 || (a.window && key0 <= tpos1 - (int32_t)a.window); };
     f16x8 qf[KF][NQ];
-    float c;
+    float c = a.c;
     {
         typename att_q<T>::raw_t qr[KF];
         float mul = 1.f, inv = 1.f;
@@ -826,7 +827,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         }
 #pragma unroll
         for (int s = 0; s < KF; s++) att_q<T>::split(qr[s], mul * a.sign, qf[s]);
-        c = att_factor(a, inv);
+        if constexpr (NQ == 2) c = att_factor(a, inv);
     }
     f32x16 o[HB];
 #pragma unroll
