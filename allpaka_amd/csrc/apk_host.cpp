@@ -1664,7 +1664,7 @@ int attend(apk_ctx* c, const char* name, const void* q, const void* k_cache, con
         a.unit = 64;
         a.heads = 1;
         block = 256;
-        shmem = (unsigned)(4 * a.unit * head_dim * 2);
+        shmem = (unsigned)(4 * a.unit * head_dim * 2 + block * 4);  // K and V of two units, a number of each lane
         kernel = "apk_attend_chunk_";
     }
     kernel += t_name + "_hd" + std::to_string(head_dim);

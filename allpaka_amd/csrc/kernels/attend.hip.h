@@ -8,11 +8,22 @@
 // Scores and outputs are held transposed (S^T = K Q^T, O^T = V^T P^T): a lane then holds one query's scores, so its
 // maximum, its sum and the rescaling of its outputs need no other lane but the two to four that share the query, and the
 // probabilities are already laid out as the second product's operand.  fp16 products are exact in f32.  With f32
-// activations a query element is the sum of two fp16 values (its row scaled by a power of two first), and so is a
-// probability: 22 bits of each take part.  With fp16 activations probabilities are rounded to fp16 once (an error of
-// 2^-11 relative at most, as that of the fp16 result).  Probabilities are 2^(x_j - r + 8), r a maximum met so far that is
-// replaced when one 2^7 times larger comes: they stay below 2^15, and a key of weight down to 2^-22 of r keeps all its bits,
-// which a long cache of small weights needs.
+// activations a query element is the sum of two fp16 values, its row scaled by a power of two first: 22 bits of it, or 2^-38 of
+// the row's largest magnitude where that is more.
+//
+// Probabilities are 2^(x_j - r + a constant), r a reference near the largest x_j, as fp16 values: below 2^16, with 11 bits from
+// 2^-14 on and steps of 2^-24 below.  What they keep of a small weight goes by where r lies:
+// * Few rows: two fp16 values, the second one 2^11 times the rest that the first leaves, its product with V added with
+//   2^-11: 22 bits, of weights down to 2^-28 of the largest key's, 2^-50 of that one below (r stays within 2 of the running
+//   maximum, at 2^14).  The launch is bound by memory: a second product costs nothing that shows (fp16 rows, 64 sequences of
+//   6000 keys: 277 us with it and without).
+// * Chunks: one fp16 value for fp16 rows (2^-11), the sum of two for f32 rows (2^-22), plain, both added up in the same place.
+//   r follows the largest x_j of the unit of keys, down as well as up: that one lies at 2^-3 at least, so that a weight that is far
+//   smaller than the largest of its unit is off by 2^-22 of that one, whatever came before.  With r the running maximum
+//   all keys behind a dominant one were held to 2^-33 of it, and where that key's value is small (a sink) nothing else is
+//   in the result.  (r moves only where a block's maximum leaves a range of 2^9 either way: 592 us for 512 tokens
+//   over 32000 keys, as with the running maximum.  A second product for fp16 rows: 944 us.  The second value scaled as for few rows in
+//   accumulators of its own: heads of 64 6 % more, of 128 43 %, of 256 three times as long, for want of registers.)
 #pragma once
 #include <type_traits>
 #include <utility>
@@ -24,7 +35,12 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-static constexpr float kProbShift = 8.0f, kMaxLag = 7.0f, kLog2e = 1.44269504088896341f;
+static constexpr float kLog2e = 1.44269504088896341f;
+// few rows: r at 2^14, moved up where a maximum is more than 2 times larger; the factor of the second values
+static constexpr float kFewShift = 14.0f, kFewLag = 1.0f, kLowUp = 2048.0f, kLowDown = 1.0f / 2048.0f;
+// chunks: r at 2^6, moved where a block's maximum is 2^9 times larger (then 2^3 below it) or smaller (then to it; not where it is
+// 2^40 below the largest one met, which counts for nothing, so that sums stay in range)
+static constexpr float kMid = 6.0f, kReach = 9.0f, kAbove = 3.0f, kDepth = 40.0f;
 #define NEG_INF (-__builtin_inff())
 
 // {lane's own value, that of lane ^ X} in some order, X = 16 or 32: one swap of half rows, no LDS.  Written out, because
@@ -555,20 +571,20 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
         f16x8 ph, pl;
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         mx = max_xor<32>(max_xor<16>(mx)) * c;
-        if (__any(mx > m + kMaxLag)) {  // the reference is moved on rarely: weights may grow to 2^kMaxLag
+        if (__any(mx > m + kFewLag)) {
             const float mn = fmaxf(m, mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < CH; i++) o[i] *= alpha;
             m = mn;
         }
-        const float sub = m == NEG_INF ? 0.f : kProbShift - m;
+        const float sub = m == NEG_INF ? 0.f : kFewShift - m;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float p = exp2_hw(__builtin_fmaf(s[j >> 2][j & 3], c, sub));
             l += p;
             ph[j] = (f16_t)p;
-            if constexpr (NQ == 2) pl[j] = (f16_t)(p - (float)ph[j]);
+            pl[j] = (f16_t)((p - (float)ph[j]) * kLowUp);
         }
         if (partial) {  // keys that no row sees: zero; values that are not finite: see below
 #pragma unroll
@@ -600,7 +616,9 @@ DEV void attend_few_body(const apk_attend_args& a, float* smem) {
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], ph, o[i], 0, 0, 0);
-            if constexpr (NQ == 2) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], pl, o[i], 0, 0, 0);
+            const f32x4 low = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], pl, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[i][j] = __builtin_fmaf(low[j], kLowDown, o[i][j]);
         }
         key0 = next;
         __builtin_amdgcn_sched_barrier(0);  // V is issued here, not at the head of the next round
@@ -890,7 +908,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             pl[b][j >> 2][(2 * j & 7) + 1] = e.y;
         }
     };
-    auto shift = [&]() { return m == NEG_INF ? 0.f : kProbShift - m; };
+    auto shift = [&]() { return m == NEG_INF ? 0.f : kMid - m; };
     auto values = [&](int b, uint32_t v_at) {
         f16x8 vf[2][2];
 #pragma unroll
@@ -907,14 +925,30 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // moves the reference on where a block's maximum asks for it; `again` redoes weights that refer to the old one
-    auto refer = [&](int b, auto&& again) {
+    // Moves the reference to where a block's maximum asks for it: down too, but for block 1 of a unit whose block 0 has
+    // weights already (PENDING), which must stay in range; `again` redoes those.  The largest maximum met at such times lies in
+    // LDS, read back by its own lane; its address is made where it is used, since kept it would cost a register all the way.
+    auto top_at = [&]() {
+        uint32_t l;
+        asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+        return (__attribute__((address_space(3))) float*)(lds + (4 * BUF + wave * 256) + l * 4);
+    };
+    *top_at() = NEG_INF;
+    auto block_max = [&](int b) {
         float mx = NEG_INF;
 #pragma unroll
         for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
-        mx = max_xor<32>(mx) * c;
-        if (__any(mx > m + kMaxLag)) {
-            const float mn = fmaxf(m, mx), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
+        return max_xor<32>(mx) * c;
+    };
+    auto refer = [&](int b, auto down_, auto pending_, auto&& again) {
+        constexpr bool DOWN = decltype(down_)::value, PENDING = decltype(pending_)::value;
+        const float mx = block_max(b), d = mx - m;
+        if (__any(DOWN ? __builtin_fabsf(d) > kReach && d != NEG_INF : d > kReach)) {
+            __attribute__((address_space(3))) float* const top = top_at();
+            const float t = *top, seen = DOWN && PENDING ? fmaxf(mx, block_max(0)) : mx;
+            const bool up = d > kReach, down = DOWN && seen < m - kReach && seen > t - kDepth;
+            *top = fmaxf(t, mx);
+            const float mn = up ? mx - kAbove : down ? seen : m, alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
             m = mn;
             again(alpha);
 #pragma unroll
@@ -977,7 +1011,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             clear(key0, buf);
             hide(0, key0);
         }
-        refer(0, [&](float alpha) { l *= alpha; });
+        refer(0, std::true_type(), std::false_type(), [&](float alpha) { l *= alpha; });
         float sub = shift();
         const float before = l;
         __builtin_amdgcn_sched_barrier(0);
@@ -993,7 +1027,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
 #pragma unroll
         for (int q = 0; q < 2; q++) vf[0][q] = load_v(0, 0, q, v_at);
         if (partial) hide(1, key0);
-        refer(1, [&](float alpha) {
+        refer(1, std::bool_constant<ANY>(), std::true_type(), [&](float alpha) {
             l = before * alpha;
             sub = shift();
 #pragma unroll
@@ -1036,7 +1070,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
 #pragma unroll
                 for (int i = 0; i < KF; i++) score(b, i, load_k(b, i, buf * BUF));
                 hide(b, key0);
-                refer(b, [&](float alpha) { l *= alpha; });
+                refer(b, std::true_type(), std::false_type(), [&](float alpha) { l *= alpha; });
                 const float sub = shift();
 #pragma unroll
                 for (int j = 0; j < 8; j++) weight(b, j, sub);

@@ -457,10 +457,12 @@ int apk_argmax_rows_noalloc(apk_ctx* ctx, const float* logits, size_t rows, size
  * The step between the K/V store and the output projection that gpu::attend / attn_block of the reference's surface
  * stand for (gpu/stub.rs; scale and window of AttnBlockReq, gpu/types.rs:302-365).
  * q, out: [n_seq][n_q*head_dim] of dtype (out may be q); k_cache, v_cache: one layer's planes; n_q a multiple of n_kv.
- * The products take all bits of fp16 and f32 queries (an f32 as the sum of two fp16), sums are f32; probabilities are
- * rounded to fp16 for fp16 rows and keep 22 bits for f32 rows.  Heads of 64, 128 and 256 run on the matrix cores; other
- * sizes up to 1024 element by element (right, and slow).  K or V rows that a row sees and that hold infinities or NaN
- * make its result infinite or NaN, in V the channels concerned; those it does not see do not reach it.
+ * Sums are f32.  Of a query the products take all bits of fp16, and 22 bits of f32 (2^-38 of the row's largest magnitude
+ * where that is more).  A key's weight keeps 22 bits (from 2^-28 of the largest on; smaller ones 2^-50 of it).  Heads of 64,
+ * 128 and 256 run on the matrix cores; other sizes up to 1024 element by element in f32 (right, and slow).
+ * Infinities and NaN in K or V that a row does not see do not reach it.  V that it sees and that is not finite makes the
+ * channels concerned infinite or NaN; NaN in K makes its row NaN.  An infinity in K counts as the formula has it (a score of
+ * +inf: the row is NaN; of -inf: weight 0), but that f32 rows may be NaN there, and a row whose scores are all -inf is zeros.
  * kv_len[s] > max_pages * page_size is cut to it, a table entry >= capacity / page_size that is needed reads page 0;
  * both raise APK_FAULT_CACHE_RANGE, and the rows of that sequence are then unspecified.
  * Uses a scratch of the context (256 MiB, allocated by the first call that may need it: inside a recording that call is
@@ -472,7 +474,9 @@ int apk_attend_paged(apk_ctx* ctx, const void* q, const void* k_cache, const voi
 /* The same for chunks: sequence s brings the rows q_off[s] .. q_off[s+1] (u32[n_seq+1], ascending, on the device; any
  * number of rows, none included), whose K and V are in the cache already: row i of m is at position kv_len[s] - m + i and
  * sees no later key (a position below 0: zeros).  Prompts, chunks of prompts over what is cached, drafts to verify, single
- * tokens, mixed in one call.  q, out: [rows][n_q*head_dim]; rows at and behind q_off[n_seq] are left as they are; a row
+ * tokens, mixed in one call.  Where sequences bring more than 16 rows times n_q / n_kv
+ * on average (and may be longer than 1024 keys, or are many), weights are held to fewer bits: for fp16 rows to 2^-11 of them, for
+ * f32 rows to 2^-22, and to 2^-22 of the largest weight of the 64 keys about them where that is more.  q, out: [rows][n_q*head_dim]; rows at and behind q_off[n_seq] are left as they are; a row
  * index > rows or a descending pair raises APK_FAULT_ROW_RANGE and is cut off.  The reference's gpu::attend_batch and the
  * attention of PrefillAttnReq (gpu/stub.rs, gpu/types.rs:302-365). */
 int apk_attend_paged_chunk(apk_ctx* ctx, const void* q, const void* k_cache, const void* v_cache, size_t capacity,
