@@ -665,8 +665,8 @@ class PageStep:
 
 class PagedCache:
     """A K/V cache shared by many sequences: region fp16 [n_planes, capacity, n_kv*head_dim] (the K and V planes of all
-    layers), in pages of page_size rows, with the page table and the lengths of n_seq sequences on the device.  The
-    methods are enqueued only, in stream order, and may be recorded (the buffers of a PageStep given to extend)."""
+    layers), in pages of page_size rows, with the page table and the lengths of n_seq sequences on the device.  Pages and
+    planes of whole 16-byte tiles only, since shared ones get copied: others are declined here.  The methods are enqueued only, in stream order, and may be recorded (the buffers of a PageStep given to extend)."""
 
     def __init__(self, backend, region, page_size, n_seq, max_pages):
         assert region.dtype == torch.float16 and region.dim() == 3 and region.is_contiguous() and region.device == backend.device
@@ -688,6 +688,9 @@ class PagedCache:
         self._state = (backend.h, _ptr(self.pool), self.n_pages, page_size, _ptr(self.page_table), max_pages, _ptr(self.kv_len), n_seq)
         planes, capacity, width = region.shape
         self._planes = (backend.h, _ptr(region), planes, capacity * width * 2, self.n_pages, page_size * width * 2)
+        # (asked for once with nothing to copy: what the library declines here it would decline after the state has changed)
+        self.b._order()
+        self._copy(_ptr(self._moves), _ptr(self._n_moves), max(n_seq, self.n_pages // 2, 1))
         self._recount()
 
     def _recount(self):

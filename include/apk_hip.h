@@ -448,7 +448,8 @@ int apk_argmax_rows_noalloc(apk_ctx* ctx, const float* logits, size_t rows, size
  * page_table: u32[n_seq][max_pages]; kv_len: u32[n_seq], the tokens a sequence holds; entries that no token needs may
  * hold anything, and so may cache rows that no sequence holds (NaN included): they are not read, or not used.  A flat
  * cache of one session is a table of one entry, 0, and page_size = capacity.  Any page_size >= 1;
- * max_pages * page_size <= 2^30; capacity < 2^32.  No counterpart in the reference, whose caches are flat (kv.rs). */
+ * max_pages * page_size <= 2^30; capacity < 2^32; pages and planes that apk_pages_copy is to serve hold whole 16-byte tiles
+ * (check before the first apk_pages_extend: its work is not undone when the copy is declined).  No counterpart in the reference, whose caches are flat (kv.rs). */
 
 /* Attention of ONE new token per sequence over the paged cache: with p = kv_len[s] - 1 (the token's own K and V are in
  * the cache already), head h of row s, and kv head g = h / (n_q / n_kv),
