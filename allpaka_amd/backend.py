@@ -55,6 +55,25 @@ def _ptr(t):
     return t.data_ptr()
 
 
+class _Queued:
+    """`with _Queued(backend): <enqueue>`: the context's stream runs after what torch has queued, and torch's current stream
+    goes on after what is enqueued here.  The context's stream and the default stream order themselves against each other;
+    any other stream of torch's is waited for, and then waits for the context's: its next work may read the results, or write
+    over an argument that was freed on it.  Inside a recording nothing runs, so nothing waits."""
+
+    __slots__ = ("backend", "follows")
+
+    def __init__(self, backend):
+        self.backend = backend
+
+    def __enter__(self):
+        self.follows = self.backend._order()
+
+    def __exit__(self, *exc):
+        if self.follows is not None:
+            self.follows.wait_stream(self.backend.stream)
+
+
 class Backend:
     """One device context (`apk_ctx`): the process-wide backend singleton of the
     reference (`with_gpu`, gpu/cuda/runtime/device.rs:944-948)."""
@@ -66,6 +85,7 @@ class Backend:
         self.h = h
         self.device = torch.device("cuda", device)
         self._recording = False
+        self._stream = None
 
     def close(self):
         if self.h:
@@ -143,12 +163,27 @@ class Backend:
         if not self._recording:
             self.sync()
 
+    @property
+    def stream(self):
+        """The stream the context launches on, as one of torch's.  The enqueue-only entries return without a wait whatever
+        torch's current stream is; with this one as the current one torch's own work follows in the same queue, where going
+        between it and the default stream costs some 50 us a time."""
+        if self._stream is None:
+            self._stream = torch.cuda.ExternalStream(self.L.apk_stream(self.h), device=self.device)
+        return self._stream
+
     def _order(self):
-        """For the enqueue-only entries: the context's stream runs after what torch has queued.  The context's stream and the
-        default stream order themselves against each other; any other stream of torch's is waited for."""
+        """For the enqueue-only entries (_Queued): waits for torch's current stream where that is needed, and returns it where
+        it has to wait for the context's in turn."""
         cur = torch.cuda.current_stream(self.device)
-        if self._recording or cur.cuda_stream not in (0, self.L.apk_stream(self.h)):
+        if self._recording:
             cur.synchronize()
+            return None
+        at = cur.cuda_stream
+        if at == 0 or at == self.L.apk_stream(self.h):
+            return None
+        cur.synchronize()
+        return cur
 
     # ---- record / replay (stream capture of gpu/cuda/prefill.rs:52-108)
     def capture_begin(self):
@@ -592,9 +627,9 @@ class Backend:
         kv_len int32 [n_seq], the token itself included; window: keys a row sees (0: all).  Enqueued only (no wait)."""
         self._attend_check(q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, out, window)
         assert q.shape[0] == kv_len.numel()
-        self._order()
-        check(self.L.apk_attend_paged(self.h, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], page_size, _ptr(page_table),
-                                      page_table.shape[1], _ptr(kv_len), kv_len.numel(), n_q, n_kv, head_dim, scale, window, _ptr(out), _dt(q)))
+        with _Queued(self):
+            check(self.L.apk_attend_paged(self.h, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], page_size, _ptr(page_table),
+                                          page_table.shape[1], _ptr(kv_len), kv_len.numel(), n_q, n_kv, head_dim, scale, window, _ptr(out), _dt(q)))
 
     def attend_paged(self, q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, scale, window=0):
         """attend_paged_into a tensor of its own, waited for."""
@@ -609,10 +644,10 @@ class Backend:
         at and behind q_off[n_seq] of out are left as they are.  Enqueued only (no wait)."""
         self._attend_check(q, k_cache, v_cache, page_size, page_table, kv_len, n_q, n_kv, head_dim, out, window)
         assert q_off.dtype == torch.int32 and q_off.numel() == kv_len.numel() + 1 and q_off.device == self.device
-        self._order()
-        check(self.L.apk_attend_paged_chunk(self.h, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], page_size, _ptr(page_table),
-                                            page_table.shape[1], _ptr(q_off), _ptr(kv_len), kv_len.numel(), q.shape[0], n_q, n_kv, head_dim,
-                                            scale, window, _ptr(out), _dt(q)))
+        with _Queued(self):
+            check(self.L.apk_attend_paged_chunk(self.h, _ptr(q), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], page_size, _ptr(page_table),
+                                                page_table.shape[1], _ptr(q_off), _ptr(kv_len), kv_len.numel(), q.shape[0], n_q, n_kv, head_dim,
+                                                scale, window, _ptr(out), _dt(q)))
 
     def attend_paged_chunk(self, q, k_cache, v_cache, page_size, page_table, q_off, kv_len, n_q, n_kv, head_dim, scale, window=0):
         """attend_paged_chunk_into a tensor of zeros, waited for."""
@@ -666,7 +701,9 @@ class PageStep:
 class PagedCache:
     """A K/V cache shared by many sequences: region fp16 [n_planes, capacity, n_kv*head_dim] (the K and V planes of all
     layers), in pages of page_size rows, with the page table and the lengths of n_seq sequences on the device.  Pages and
-    planes of whole 16-byte tiles only, since shared ones get copied: others are declined here.  The methods are enqueued only, in stream order, and may be recorded (the buffers of a PageStep given to extend)."""
+    planes of whole 16-byte tiles only, since shared ones get copied: others are declined here.  The methods are enqueued
+    only, on the context's stream: after what torch's current stream holds, and before what it gets next (Backend.stream).
+    They may be recorded (the buffers of a PageStep given to extend)."""
 
     def __init__(self, backend, region, page_size, n_seq, max_pages):
         assert region.dtype == torch.float16 and region.dim() == 3 and region.is_contiguous() and region.device == backend.device
@@ -689,13 +726,13 @@ class PagedCache:
         planes, capacity, width = region.shape
         self._planes = (backend.h, _ptr(region), planes, capacity * width * 2, self.n_pages, page_size * width * 2)
         # (asked for once with nothing to copy: what the library declines here it would decline after the state has changed)
-        self.b._order()
-        self._copy(_ptr(self._moves), _ptr(self._n_moves), max(n_seq, self.n_pages // 2, 1))
+        with _Queued(backend):
+            self._copy(_ptr(self._moves), _ptr(self._n_moves), max(n_seq, self.n_pages // 2, 1))
         self._recount()
 
     def _recount(self):
-        self.b._order()
-        check(self.b.L.apk_pages_init(*self._state))
+        with _Queued(self.b):
+            check(self.b.L.apk_pages_init(*self._state))
 
     @property
     def refs(self):
@@ -730,8 +767,8 @@ class PagedCache:
     def restore(self, saved):
         """The state of a save again."""
         assert saved.dtype == torch.int32 and saved.device == self.b.device and saved.numel() == self._all.numel()
-        self.b._order()
-        check(self.b.L.apk_copy(self.b.h, _ptr(saved), self._all.data_ptr(), 4 * self._all.numel()))
+        with _Queued(self.b):
+            check(self.b.L.apk_copy(self.b.h, _ptr(saved), self._all.data_ptr(), 4 * self._all.numel()))
 
     def _ids(self, t, n=None):
         assert t.dtype == torch.int32 and t.device == self.b.device and (n is None or t.numel() == n)
@@ -743,28 +780,28 @@ class PagedCache:
         assert step is not None or not self.b._recording, "a recording needs a step that outlives it"
         step = PageStep(self.n_seq, rows, self.b.device) if step is None else step
         assert step.rows == rows and step.n_seq == self.n_seq
-        self.b._order()
         q_off, positions, slots, pairs, n_pairs = step._ptrs
-        check(self.b.L.apk_pages_extend(*self._state, self._ids(n_new, self.n_seq), rows, q_off, positions, slots, pairs, n_pairs))
-        self._copy(pairs, n_pairs, self.n_seq)
+        with _Queued(self.b):
+            check(self.b.L.apk_pages_extend(*self._state, self._ids(n_new, self.n_seq), rows, q_off, positions, slots, pairs, n_pairs))
+            self._copy(pairs, n_pairs, self.n_seq)
         return step
 
     def fork(self, src, dst):
         """Sequences dst (holding nothing) become further holders of the pages of sequences src."""
         assert src.numel() == dst.numel()
-        self.b._order()
-        check(self.b.L.apk_pages_fork(*self._state, self._ids(src), self._ids(dst), src.numel()))
+        with _Queued(self.b):
+            check(self.b.L.apk_pages_fork(*self._state, self._ids(src), self._ids(dst), src.numel()))
 
     def truncate(self, new_len):
         """Cuts sequences to new_len int32 [n_seq] tokens; -1 leaves one as it is, 0 frees it."""
-        self.b._order()
-        check(self.b.L.apk_pages_truncate(*self._state, self._ids(new_len, self.n_seq)))
+        with _Queued(self.b):
+            check(self.b.L.apk_pages_truncate(*self._state, self._ids(new_len, self.n_seq)))
 
     def compact(self):
         """Moves the pages in use to the front of every plane."""
-        self.b._order()
-        check(self.b.L.apk_pages_compact(*self._state, _ptr(self._moves), _ptr(self._n_moves)))
-        self._copy(_ptr(self._moves), _ptr(self._n_moves), max(self.n_pages // 2, 1))
+        with _Queued(self.b):
+            check(self.b.L.apk_pages_compact(*self._state, _ptr(self._moves), _ptr(self._n_moves)))
+            self._copy(_ptr(self._moves), _ptr(self._n_moves), max(self.n_pages // 2, 1))
 
     def _copy(self, pairs, n_pairs, most):
         check(self.b.L.apk_pages_copy(*self._planes, pairs, n_pairs, most))

@@ -34,7 +34,7 @@ class Host(backend.Backend):
     """A Backend without a device."""
 
     def __init__(self):
-        self.L, self.h, self.device, self._recording = Library(), 1, torch.device("cpu"), False
+        self.L, self.h, self.device, self._recording, self._stream = Library(), 1, torch.device("cpu"), False, None
 
     def close(self):
         pass
@@ -76,3 +76,97 @@ def test_pages_of_whole_tiles_are_taken(be):
         c = backend.PagedCache(be, region(planes, rows, width), page, 3, 4)
         c.extend(torch.zeros(3, dtype=torch.int32), 5)
         c.compact()
+
+
+class Stream:
+    def __init__(self, handle, log):
+        self.cuda_stream, self.log = handle, log
+
+    def synchronize(self):
+        self.log.append("host waits")
+
+    def wait_stream(self, other):
+        self.log.append(("waits for", other.cuda_stream))
+
+
+CONTEXT, SIDE = 4000, 7000
+
+
+@pytest.fixture
+def streams(be, monkeypatch):
+    """be with a stream of its own; streams(handle) makes torch's current one."""
+    log = be.L.calls
+    monkeypatch.setattr(type(be.L), "apk_stream", lambda self, ctx: CONTEXT, raising=False)
+    monkeypatch.setattr(Host, "_order", backend.Backend._order)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: Stream(handle, log))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(0, log))
+
+    def current(handle):
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(handle, log))
+        log.clear()
+        return log
+
+    return current
+
+
+def entries(be):
+    """name -> (a call, what it enqueues last)"""
+    cache = backend.PagedCache(be, region(2, 64, 16), 16, 3, 4)
+    ids, state = torch.zeros(3, dtype=torch.int32), torch.zeros_like(cache._all)
+    q = torch.zeros((3, 32), dtype=torch.float16)
+    off = torch.zeros(4, dtype=torch.int32)
+    step = backend.PageStep(3, 5, be.device)
+    paged = (cache.region[0], cache.region[1], 16, cache.page_table)
+    return {
+        "extend": (lambda: cache.extend(ids, 5, step), "copy"),
+        "fork": (lambda: cache.fork(ids, ids), "apk_pages_fork"),
+        "truncate": (lambda: cache.truncate(ids), "apk_pages_truncate"),
+        "compact": (lambda: cache.compact(), "copy"),
+        "restore": (lambda: cache.restore(state), "apk_copy"),
+        "adopt": (lambda: cache.adopt(cache.page_table.clone(), cache.kv_len.clone()), "apk_pages_init"),
+        "new": (lambda: backend.PagedCache(be, cache.region, 16, 3, 4), "apk_pages_init"),
+        "tokens": (lambda: be.attend_paged_into(q, *paged, cache.kv_len, 2, 1, 16, 1.0, q), "apk_attend_paged"),
+        "chunk": (lambda: be.attend_paged_chunk_into(q, *paged, off, cache.kv_len, 2, 1, 16, 1.0, q), "apk_attend_paged_chunk"),
+    }
+
+
+NAMES = ["extend", "fork", "truncate", "compact", "restore", "adopt", "new", "tokens", "chunk"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_side_stream_comes_before_and_after_what_is_enqueued(be, streams, name):
+    """What the side stream does next may read the results, or write over an argument that was freed there."""
+    call, last = entries(be)[name]
+    log = streams(SIDE)
+    call()
+    first = min(i for i, x in enumerate(log) if x == "copy" or str(x).startswith(("apk_pages", "apk_attend", "apk_copy")))
+    assert "host waits" in log[:first]
+    assert log[-1] == ("waits for", CONTEXT) and log[-2] == last, log
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("handle", [0, CONTEXT])
+def test_the_default_stream_and_the_context_s_own_need_no_wait(be, streams, name, handle):
+    call, last = entries(be)[name]
+    log = streams(handle)
+    call()
+    assert log[-1] == last and not any(isinstance(x, tuple) for x in log), log
+
+
+@pytest.mark.parametrize("name", [n for n in NAMES if n != "adopt"])
+def test_nothing_waits_for_a_recording(be, streams, name):
+    call, last = entries(be)[name]
+    log = streams(SIDE)
+    be._recording = True
+    call()
+    assert log[-1] == last and not any(isinstance(x, tuple) for x in log), log
+
+
+@pytest.mark.parametrize("name", ["extend", "compact"])
+def test_a_side_stream_waits_also_where_the_copy_fails(be, streams, name):
+    call, _ = entries(be)[name]
+    be.L.apk_pages_copy = lambda *a: DECLINE_SHAPE
+    log = streams(SIDE)
+    with pytest.raises(Declined):
+        call()
+    assert log[-1] == ("waits for", CONTEXT), log
