@@ -825,7 +825,9 @@ class Graph:
         return n.value
 
     def launch(self):
-        check(self.be.L.apk_graph_launch(self.be.h, self.g))
+        """Enqueued only, as a step of the paged cache is."""
+        with _Queued(self.be):
+            check(self.be.L.apk_graph_launch(self.be.h, self.g))
 
     def destroy(self):
         if self.g:

@@ -117,3 +117,33 @@ def test_torch_on_the_context_s_own_stream(be, busy):
         got = out.float() * 2
     be.sync()
     assert np.all(np.abs(got.cpu().numpy() / 2 - want) <= tol)
+
+
+def test_a_recorded_step_replayed_from_a_side_stream(be, busy):
+    """Its arguments are written, and its results read, by the side stream's own work."""
+    import allpaka_amd as apk
+
+    n_seq, rows = 3, 8
+    region = torch.zeros((2, 40 * 4, 8), dtype=torch.float16, device="cuda")
+    cache, model = apk.PagedCache(be, region, 4, n_seq, 8), PageModel(40, 4, n_seq, 8)
+    n_new, step = i32([0] * n_seq), apk.backend.PageStep(n_seq, rows, be.device)
+    cache.extend(n_new, rows, step)
+    with be.record() as rec:
+        cache.extend(n_new, rows, step)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    seen = []
+    try:
+        with torch.cuda.stream(side):
+            for news in ([3, 1, 0], [1, 1, 1], [0, 2, 5], [1, 0, 1]):
+                n_new.copy_(i32(news))
+                busy()
+                rec.graph.launch()
+                seen.append((step.slots.clone(), cache.kv_len.clone(), model.extend(news, rows)[2], list(model.kv_len)))
+        side.synchronize()
+        for slots, lens, want, want_lens in seen:
+            assert slots.cpu().numpy().view(np.uint32).tolist() == want + [2 ** 32 - 1] * (rows - len(want))
+            assert lens.cpu().tolist() == want_lens
+        assert be.take_faults() == 0
+    finally:
+        rec.graph.destroy()

@@ -127,10 +127,11 @@ def entries(be):
         "new": (lambda: backend.PagedCache(be, cache.region, 16, 3, 4), "apk_pages_init"),
         "tokens": (lambda: be.attend_paged_into(q, *paged, cache.kv_len, 2, 1, 16, 1.0, q), "apk_attend_paged"),
         "chunk": (lambda: be.attend_paged_chunk_into(q, *paged, off, cache.kv_len, 2, 1, 16, 1.0, q), "apk_attend_paged_chunk"),
+        "replay": (lambda: backend.Graph(be, 5).launch(), "apk_graph_launch"),
     }
 
 
-NAMES = ["extend", "fork", "truncate", "compact", "restore", "adopt", "new", "tokens", "chunk"]
+NAMES = ["extend", "fork", "truncate", "compact", "restore", "adopt", "new", "tokens", "chunk", "replay"]
 
 
 @pytest.mark.parametrize("name", NAMES)
@@ -139,7 +140,7 @@ def test_a_side_stream_comes_before_and_after_what_is_enqueued(be, streams, name
     call, last = entries(be)[name]
     log = streams(SIDE)
     call()
-    first = min(i for i, x in enumerate(log) if x == "copy" or str(x).startswith(("apk_pages", "apk_attend", "apk_copy")))
+    first = min(i for i, x in enumerate(log) if x == "copy" or str(x).startswith(("apk_pages", "apk_attend", "apk_copy", "apk_graph")))
     assert "host waits" in log[:first]
     assert log[-1] == ("waits for", CONTEXT) and log[-2] == last, log
 
@@ -153,7 +154,7 @@ def test_the_default_stream_and_the_context_s_own_need_no_wait(be, streams, name
     assert log[-1] == last and not any(isinstance(x, tuple) for x in log), log
 
 
-@pytest.mark.parametrize("name", [n for n in NAMES if n != "adopt"])
+@pytest.mark.parametrize("name", [n for n in NAMES if n not in ("adopt", "replay")])
 def test_nothing_waits_for_a_recording(be, streams, name):
     call, last = entries(be)[name]
     log = streams(SIDE)
