@@ -430,7 +430,7 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_truncate_k(uint
             if (held == 1) {
                 __hip_atomic_fetch_or(P.bits + e / 32, 1u << (e & 31), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 atomicAdd(&freed, 1u);
-            } else if (held == 0) {  // nobody held it: the table does not belong to this pool
+            } else if ((int32_t)held <= 0) {  // nobody held it (below 0: so others found, and have not put theirs back yet)
                 pg_add(P.refs + e, 1);
                 atomicOr(fault, APK_FAULT_CACHE_RANGE);
             }
