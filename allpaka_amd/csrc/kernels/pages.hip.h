@@ -106,6 +106,9 @@ DEV uint32_t pg_find(const uint32_t* off, uint32_t n, uint32_t k) {
     return lo;
 }
 DEV uint32_t pg_ceil(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+// Sequences that a round over tables takes, a lane each: as many as have fewer than 2^31 entries between them, so that neither
+// their sum nor an index that steps past it leaves 32 bits.
+DEV uint32_t pg_round(uint32_t max_pages) { return min((uint32_t)PG_BLOCK, 0x7fffffffu / max(max_pages, 1u)); }
 
 // The pool counted afresh from the page tables (n_seq 0: every page free).
 extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_init_k(uint32_t* pool, uint32_t n_pages, uint32_t page, const uint32_t* table,
@@ -396,10 +399,11 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_truncate_k(uint
     const uint32_t tid = threadIdx.x;
     __shared__ uint32_t sm[PG_BLOCK / 64 + 1], freed, off[PG_BLOCK], s_keep[PG_BLOCK];
     if (tid == 0) freed = 0;
-    for (uint32_t base = 0; base < n_seq; base += PG_BLOCK) {
-        const uint32_t s = base + tid, here = min((uint32_t)PG_BLOCK, n_seq - base);
+    const uint32_t round = pg_round(max_pages);
+    for (uint32_t base = 0; base < n_seq; base += round) {
+        const uint32_t s = base + tid, here = min(round, n_seq - base);
         uint32_t gone = 0, keep = 0;
-        if (s < n_seq) {
+        if (tid < here) {
             const uint32_t len = kv_len[s], cut = new_len[s];
             if (cut < len) {
                 uint32_t have = pg_ceil(len, page);
@@ -500,9 +504,10 @@ extern "C" __global__ __launch_bounds__(PG_BLOCK) void apk_pages_compact_k(uint3
     }
     pg_sync();
     if (moves) {
-        for (uint32_t base = 0; base < n_seq; base += PG_BLOCK) {
-            const uint32_t s = base + tid, here = min((uint32_t)PG_BLOCK, n_seq - base);
-            const uint32_t used = s < n_seq ? min(pg_ceil(kv_len[s], page), max_pages) : 0;
+        const uint32_t round = pg_round(max_pages);
+        for (uint32_t base = 0; base < n_seq; base += round) {
+            const uint32_t s = base + tid, here = min(round, n_seq - base);
+            const uint32_t used = tid < here ? min(pg_ceil(kv_len[s], page), max_pages) : 0;
             uint32_t all;
             const uint32_t inc = pg_scan(used, sm, all);
             if (tid < here) off[tid] = inc - used;
