@@ -21,9 +21,12 @@
 //   r follows the largest x_j of the unit of keys, down as well as up: that one lies at 2^-3 at least, so that a weight that is far
 //   smaller than the largest of its unit is off by 2^-22 of that one, whatever came before.  With r the running maximum
 //   all keys behind a dominant one were held to 2^-33 of it, and where that key's value is small (a sink) nothing else is
-//   in the result.  (r moves only where a block's maximum leaves a range of 2^9 either way: 592 us for 512 tokens
-//   over 32000 keys, as with the running maximum.  A second product for fp16 rows: 944 us.  The second value scaled as for few rows in
-//   accumulators of its own: heads of 64 6 % more, of 128 43 %, of 256 three times as long, for want of registers.)
+//   in the result.  r comes down at once the first times and once in 8 units then, so that scores that jump up and down
+//   all along do not cost a rescaling each time; they are held to 2^-33 of the largest meanwhile.  (512 tokens over 32000 keys,
+//   us with the running maximum / this way: fp16, heads of 64 420 / 420, of 128 596 / 601, of 256 1480 / 1479, f32 of 128 998 / 989;
+//   with scores three times as wide 604 / 615 and 983 / 1024; coming down freely 677 and 1197 there.  A second product for
+//   fp16 rows: 944 for 603.  The second value scaled as for few rows, in accumulators of its own: f32 heads of 64 6 % more, of
+//   128 43 %, of 256 three times as long, for want of registers.)
 #pragma once
 #include <type_traits>
 #include <utility>
@@ -38,9 +41,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 static constexpr float kLog2e = 1.44269504088896341f;
 // few rows: r at 2^14, moved up where a maximum is more than 2 times larger; the factor of the second values
 static constexpr float kFewShift = 14.0f, kFewLag = 1.0f, kLowUp = 2048.0f, kLowDown = 1.0f / 2048.0f;
-// chunks: r at 2^6, moved where a block's maximum is 2^9 times larger (then 2^3 below it) or smaller (then to it; not where it is
-// 2^40 below the largest one met, which counts for nothing, so that sums stay in range)
-static constexpr float kMid = 6.0f, kReach = 9.0f, kAbove = 3.0f, kDepth = 40.0f;
+// chunks: r at 2^6.  Where a block's maximum is 2^9 times larger r moves to 2^2 below it, where it is 2^9 times smaller to 2^6
+// above it (the next ones may be larger); not down to one 2^40 below the largest met, which counts for nothing, so that sums
+// stay in range.  A move takes 8 units of keys from an account that begins with three moves; down only what is on it.
+static constexpr float kMid = 6.0f, kReach = 9.0f, kAbove = 2.0f, kRoom = 6.0f, kDepth = 40.0f;
+static constexpr int32_t kMoves = 3, kMoveUnits = 8;
 #define NEG_INF (-__builtin_inff())
 
 // {lane's own value, that of lane ^ X} in some order, X = 16 or 32: one swap of half rows, no LDS.  Written out, because
@@ -925,30 +930,31 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Moves the reference to where a block's maximum asks for it: down too, but for block 1 of a unit whose block 0 has
-    // weights already (PENDING), which must stay in range; `again` redoes those.  The largest maximum met at such times lies in
-    // LDS, read back by its own lane; its address is made where it is used, since kept it would cost a register all the way.
+    // Moves the reference to where block b of unit u asks for it, up or down; `again` redoes what refers to the old one.  Not
+    // down (DOWN false) for block 1 where block 0 has weights already, which must stay in range: a row that sees block 0 has a
+    // reference by it, and one that does not has none yet.  The largest maximum met at such times lies in LDS, read back by
+    // its own lane; its address is made where it is used, since kept it would cost a register all the way.
     auto top_at = [&]() {
         uint32_t l;
         asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
         return (__attribute__((address_space(3))) float*)(lds + (4 * BUF + wave * 256) + l * 4);
     };
     *top_at() = NEG_INF;
-    auto block_max = [&](int b) {
+    int32_t spent = (int32_t)sp.u0 - kMoves * kMoveUnits;
+    auto refer = [&](uint32_t u, int b, auto down_, auto&& again) {
+        constexpr bool DOWN = decltype(down_)::value;
         float mx = NEG_INF;
 #pragma unroll
         for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
-        return max_xor<32>(mx) * c;
-    };
-    auto refer = [&](int b, auto down_, auto pending_, auto&& again) {
-        constexpr bool DOWN = decltype(down_)::value, PENDING = decltype(pending_)::value;
-        const float mx = block_max(b), d = mx - m;
-        if (__any(DOWN ? __builtin_fabsf(d) > kReach && d != NEG_INF : d > kReach)) {
+        mx = max_xor<32>(mx) * c;
+        const float d = mx - m, below = (int32_t)u - spent >= kMoveUnits ? -kReach : NEG_INF;
+        const bool low = DOWN && d < below && d != NEG_INF;  // (-inf: a row that sees nothing of the block)
+        if (__builtin_expect(__any(d > kReach || low), 0)) {
+            spent += kMoveUnits;
             __attribute__((address_space(3))) float* const top = top_at();
-            const float t = *top, seen = DOWN && PENDING ? fmaxf(mx, block_max(0)) : mx;
-            const bool up = d > kReach, down = DOWN && seen < m - kReach && seen > t - kDepth;
+            const float t = *top;
             *top = fmaxf(t, mx);
-            const float mn = up ? mx - kAbove : down ? seen : m, alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
+            const float mn = low && mx > t - kDepth ? mx + kRoom : fmaxf(m, mx - kAbove), alpha = mn == NEG_INF ? 1.f : exp2_hw(m - mn);
             m = mn;
             again(alpha);
 #pragma unroll
@@ -1011,7 +1017,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
             clear(key0, buf);
             hide(0, key0);
         }
-        refer(0, std::true_type(), std::false_type(), [&](float alpha) { l *= alpha; });
+        refer(u, 0, std::true_type(), [&](float alpha) { l *= alpha; });
         float sub = shift();
         const float before = l;
         __builtin_amdgcn_sched_barrier(0);
@@ -1027,7 +1033,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
 #pragma unroll
         for (int q = 0; q < 2; q++) vf[0][q] = load_v(0, 0, q, v_at);
         if (partial) hide(1, key0);
-        refer(1, std::bool_constant<ANY>(), std::true_type(), [&](float alpha) {
+        refer(u, 1, std::false_type(), [&](float alpha) {
             l = before * alpha;
             sub = shift();
 #pragma unroll
@@ -1070,7 +1076,7 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
 #pragma unroll
                 for (int i = 0; i < KF; i++) score(b, i, load_k(b, i, buf * BUF));
                 hide(b, key0);
-                refer(b, std::true_type(), std::false_type(), [&](float alpha) { l *= alpha; });
+                refer(u, b, std::true_type(), [&](float alpha) { l *= alpha; });
                 const float sub = shift();
 #pragma unroll
                 for (int j = 0; j < 8; j++) weight(b, j, sub);

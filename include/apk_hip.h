@@ -477,7 +477,8 @@ int apk_attend_paged(apk_ctx* ctx, const void* q, const void* k_cache, const voi
  * sees no later key (a position below 0: zeros).  Prompts, chunks of prompts over what is cached, drafts to verify, single
  * tokens, mixed in one call.  Where sequences bring more than 16 rows times n_q / n_kv
  * on average (and may be longer than 1024 keys, or are many), weights are held to fewer bits: for fp16 rows to 2^-11 of them, for
- * f32 rows to 2^-22, and to 2^-22 of the largest weight of the 64 keys about them where that is more.  q, out: [rows][n_q*head_dim]; rows at and behind q_off[n_seq] are left as they are; a row
+ * f32 rows to 2^-22, and to 2^-22 of the largest weight of the 64 keys about them where that is more (of weights that rise
+ * and fall by more than 2^9 several times within a few hundred keys: to 2^-33 of the row's largest).  q, out: [rows][n_q*head_dim]; rows at and behind q_off[n_seq] are left as they are; a row
  * index > rows or a descending pair raises APK_FAULT_ROW_RANGE and is cut off.  The reference's gpu::attend_batch and the
  * attention of PrefillAttnReq (gpu/stub.rs, gpu/types.rs:302-365). */
 int apk_attend_paged_chunk(apk_ctx* ctx, const void* q, const void* k_cache, const void* v_cache, size_t capacity,
