@@ -1085,7 +1085,9 @@ DEV void attend_chunk_body(const apk_attend_args& a, char* smem) {
         }
         lds_arrived();
     };
-    // units [f0, f1), an even number, are seen whole by all rows
+    // Units [f0, f1), an even number, are seen whole by all rows.  A wave without rows takes them by part_seen next to the
+    // others' `whole`: both have to meet the same barriers there.  They do: one each at the end, and none in `clear`, which
+    // runs only in units that some row does not see whole, for all waves or none.
     int32_t w0 = a.window ? tpos1 - (int32_t)a.window + 1 : 0, w1 = tpos0 + 1;
     uint32_t f0 = max(sp.u0, (uint32_t)max(0, (max(w0, sp.lo) + BN - 1) / BN)), f1 = min(sp.u1, (uint32_t)max(0, w1 / BN));
     f0 = min(f0, sp.u1);
