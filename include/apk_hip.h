@@ -459,8 +459,9 @@ int apk_argmax_rows_noalloc(apk_ctx* ctx, const float* logits, size_t rows, size
  * stand for (gpu/stub.rs; scale and window of AttnBlockReq, gpu/types.rs:302-365).
  * q, out: [n_seq][n_q*head_dim] of dtype (out may be q); k_cache, v_cache: one layer's planes; n_q a multiple of n_kv.
  * Sums are f32.  Of a query the products take all bits of fp16, and 22 bits of f32 (2^-38 of the row's largest magnitude
- * where that is more).  A key's weight keeps 22 bits (from 2^-28 of the largest on; smaller ones 2^-50 of it).  Heads of 64,
- * 128 and 256 run on the matrix cores; other sizes up to 1024 element by element in f32 (right, and slow).
+ * where that is more).  A key's weight keeps 22 bits (from 2^-28 of the largest on; smaller ones 2^-50 of it);
+ * with n_q / n_kv above 16 it may keep what weights of chunks keep, see there.  Heads of 64, 128 and 256 run on the matrix
+ * cores; other sizes up to 1024 element by element in f32 (right, and slow).
  * Infinities and NaN in K or V that a row does not see do not reach it.  V that it sees and that is not finite makes the
  * channels concerned infinite or NaN; NaN in K makes its row NaN.  An infinity in K counts as the formula has it (a score of
  * +inf: the row is NaN; of -inf: weight 0), but that f32 rows may be NaN there, and a row whose scores are all -inf is zeros.

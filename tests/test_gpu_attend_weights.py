@@ -192,3 +192,22 @@ def test_levels_that_alternate(be, hd, f16, bits):
     err = np.abs(attend(be, c, 1.0, 0, True, dev(c["V"])) - want)
     # (each of them off by 2^-33, times its value, over the sum of the weights)
     assert np.all(err <= rel * want + 1.5 * 2.0 ** -33 + (2.0 ** -25 if f16 else 0)), f"worst {np.max(err) / want:.2e} of the result"
+
+
+# Scores of widths from the ordinary to next to one-hot, random, so that the reference of the weights moves at any place: in units
+# seen in part and whole, at windows' ends and in odd parts; and a key that outweighs all, first, in the middle or last.
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("gain", [4.0, 12.0, 40.0])
+@pytest.mark.parametrize("hd,n_q,n_kv,page,window", [(64, 6, 2, 24, 0), (128, 4, 1, 16, 700), (256, 2, 1, 33, 0), (256, 3, 1, 16, 500), (128, 40, 1, 64, 0)])
+def test_wide_scores(be, f16, gain, hd, n_q, n_kv, page, window):
+    from tests.paged_util import attention64
+
+    seqs = [(1100, 60), (3, 90), (2500, 2)]
+    c = make_case(830 + hd + window, [a + b for a, b in seqs], [b for _, b in seqs], n_q, n_kv, hd, page, f16, q_gain=gain)
+    for s, j in ((0, 0), (0, 640), (1, 92)):
+        at = c["table"][s][j // page] * page + j % page
+        c["K"][at, :hd] = 3.0 * np.sign(c["q"][c["q_off"][s], :hd]).astype(np.float16)
+    want, tol = attention64(c, hd ** -0.5, window)
+    got = attend(be, c, hd ** -0.5, window, True, dev(c["V"]))
+    err = np.abs(got - want)
+    assert np.all(err <= tol), f"worst {np.max(err / tol):.2f} of the bound"
