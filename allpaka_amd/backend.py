@@ -704,7 +704,8 @@ class PagedCache:
     layers), in pages of page_size rows, with the page table and the lengths of n_seq sequences on the device.  Pages and
     planes of whole 16-byte tiles only, since shared ones get copied: others are declined here.  The methods are enqueued
     only, on the context's stream: after what torch's current stream holds, and before what it gets next (Backend.stream).
-    They may be recorded (the buffers of a PageStep given to extend)."""
+    They may be recorded (the buffers of a PageStep given to extend).  One host thread at a time: extend and compact are
+    two launches, and between them the tables name pages that are yet to be copied."""
 
     def __init__(self, backend, region, page_size, n_seq, max_pages):
         assert region.dtype == torch.float16 and region.dim() == 3 and region.is_contiguous() and region.device == backend.device
